@@ -19,7 +19,7 @@
  *     [0, vocab), a bounded wait that ran out) are OR-ed as TOME_DEV_* bits into the
  *     optional caller-owned `dev_status` word (device memory, int32, zero it before
  *     the first call; nullable); kernels never trap;
- *   - dtype codes: TOME_F32 = 0, TOME_BF16 = 1;
+ *   - dtype codes: TOME_F32 = 0, TOME_BF16 = 1, TOME_F16 = 2 (accepted where an entry point says so);
  *   - all index arithmetic is 64-bit.
  */
 #ifndef TOME_B200_H_
@@ -34,7 +34,7 @@ extern "C" {
 
 #define TOME_B200_VERSION 100
 
-enum tome_dtype { TOME_F32 = 0, TOME_BF16 = 1 };
+enum tome_dtype { TOME_F32 = 0, TOME_BF16 = 1, TOME_F16 = 2 };
 
 enum tome_status {
   TOME_OK = 0,
@@ -56,6 +56,7 @@ enum tome_status {
 #define TOME_DEV_RAGGED_OVERFLOW 4 /* windows cover more positions than the packed arrays hold */
 #define TOME_DEV_BLOCK_OUT_OF_RANGE 8 /* a block-table entry outside [0, num_blocks) */
 #define TOME_DEV_NO_CANDIDATE 16 /* sampling: a row without a single logit that is not NaN */
+#define TOME_DEV_POSITION_OUT_OF_RANGE 32 /* a position outside the rotary table */
 
 /* Library version (TOME_B200_VERSION of the build). */
 int32_t tome_version(void);
@@ -325,6 +326,143 @@ int32_t tome_combine_triples(const float* m, const float* s, int64_t ms_part_str
                              int32_t n_parts, const float* t, int64_t t_part_stride,
                              int32_t n_t_parts, int64_t rows, float* out_logprob,
                              float* out_lse, void* stream);
+
+/*
+ * Norms of queries and keys for each head with the rotary position rotation, in one pass
+ * (the reference's kernel: mlx-impl/model.py:105-194; there it feeds mlx-impl/model.py:410-421).
+ * For each token and head x of head_dim elements, in fp32 and rounded once on the store:
+ *   y = x * rsqrt(mean(x^2) + eps) * weight, then with (cos, sin) of the token's position
+ *   z[i] = y[i] cos[i] - y[i + D/2] sin[i],  z[i + D/2] = y[i + D/2] cos[i] + y[i] sin[i].
+ *
+ *   qkv        device [tokens, (heads + 2 kv_heads) * head_dim], the fused projection's output
+ *              (queries, keys, values of a token side by side); token t starts at element
+ *              t * qkv_stride (qkv_stride >= the width, rows on 16-byte boundaries)
+ *   dtype      TOME_F32, TOME_BF16 or TOME_F16; the weights and outputs have it too
+ *   head_dim   a multiple of 16 in [16, 256]
+ *   cos_sin    device fp32 [n_positions, head_dim]: cos of the head_dim / 2 angles, then their sin
+ *   positions  device int32 [tokens]; one outside [0, n_positions) gives NaN and sets
+ *              TOME_DEV_POSITION_OUT_OF_RANGE
+ *   q_out      [tokens, heads, head_dim]; k_out [tokens, kv_heads, head_dim]; the values are not
+ *              touched.  All tensors 16-byte aligned; outputs may not overlap inputs.
+ */
+int32_t tome_qk_norm_rope(const void* qkv, int32_t dtype, int64_t tokens, int32_t heads,
+                          int32_t kv_heads, int32_t head_dim, int64_t qkv_stride,
+                          const void* q_weight, const void* k_weight, const float* cos_sin,
+                          int32_t n_positions, const int32_t* positions, float eps, void* q_out,
+                          void* k_out, int32_t* dev_status, void* stream);
+
+/*
+ * The same for serving: the keys (normed and rotated) and the values (as they are) of token t go
+ * to the paged pools of tome_gather_paged_kv instead, at place cache_positions[t] of sequence
+ * seq_ids[t] (NULL: token t is sequence t's, n_seq = tokens):
+ *   pool[block_tables[seq, at / block_size], h, at % block_size, :].
+ * Unlike tome_update_paged_kv it writes anywhere in a block, so a decode step appends one token.
+ * cache_positions[t] < 0: the token is not cached.  A place that the table or the pool does not
+ * have is skipped and sets TOME_DEV_BLOCK_OUT_OF_RANGE; a token whose position is bad gets NaN
+ * queries and no key.  Two tokens of a call that name one place race.
+ */
+int32_t tome_qk_norm_rope_append(const void* qkv, int32_t dtype, int64_t tokens, int32_t heads,
+                                 int32_t kv_heads, int32_t head_dim, int64_t qkv_stride,
+                                 const void* q_weight, const void* k_weight, const float* cos_sin,
+                                 int32_t n_positions, const int32_t* positions, float eps,
+                                 const int32_t* seq_ids, const int32_t* block_tables,
+                                 const int32_t* cache_positions, int64_t n_seq, int32_t block_size,
+                                 int32_t max_blocks, int32_t num_blocks, void* q_out, void* k_pool,
+                                 void* v_pool, int32_t* dev_status, void* stream);
+
+/*
+ * Backward of tome_qk_norm_rope (no counterpart in the reference, which does not train):
+ *   grad_q, grad_k  device, the gradients of q_out and k_out, contiguous
+ *   grad_v     device [tokens, kv_heads, head_dim], copied into the value part of grad_qkv, or
+ *              NULL: that part is written as zeros
+ *   grad_qkv   device [tokens, (heads + 2 kv_heads) * head_dim], contiguous
+ *   grad_q_weight, grad_k_weight  device fp32 [head_dim], summed over tokens and heads in an
+ *              order that depends on the sizes alone
+ *   workspace  device scratch of tome_qk_norm_rope_backward_workspace_bytes, 16-byte aligned; needs
+ *              no initialisation
+ */
+size_t tome_qk_norm_rope_backward_workspace_bytes(int32_t head_dim);
+int32_t tome_qk_norm_rope_backward(const void* grad_q, const void* grad_k, const void* grad_v,
+                                   const void* qkv, int32_t dtype, int64_t tokens, int32_t heads,
+                                   int32_t kv_heads, int32_t head_dim, int64_t qkv_stride,
+                                   const void* q_weight, const void* k_weight,
+                                   const float* cos_sin, int32_t n_positions,
+                                   const int32_t* positions, float eps, void* grad_qkv,
+                                   float* grad_q_weight, float* grad_k_weight, void* workspace,
+                                   size_t workspace_bytes, int32_t* dev_status, void* stream);
+
+/*
+ * Single-token attention over the paged pools for a batch whose sequences share prefixes: the
+ * sequences [group_starts[g], group_starts[g + 1]) attend to the first prefix_lens[g] tokens of
+ * the pages in prefix_tables[g], which are read once for all of them, and each sequence b to the
+ * first lengths[b] tokens of its own pages in block_tables[b].  (The reference copies the
+ * prefix for every completion: mlx-impl/node.py:529-555, and attends over the whole:
+ * mlx-impl/model.py:428.)
+ *
+ *   q          device [n_seq, heads, head_dim], TOME_BF16 or TOME_F16, sequence stride q_stride
+ *              elements (16-byte rows); KV head of query head h: h / (heads / kv_heads);
+ *              heads / kv_heads <= 128; head_dim 64 or 128
+ *   k_pool, v_pool  device [num_blocks, kv_heads, block_size, head_dim], the type of q
+ *   prefix_tables  device int32 [n_groups, prefix_blocks]; prefix_lens int32 [n_groups]
+ *   group_starts   device int32 [n_groups + 1], not decreasing; sequences outside
+ *              [group_starts[0], group_starts[n_groups]) have no prefix (n_groups 0: none has)
+ *   block_tables   device int32 [n_seq, max_blocks]; lengths int32 [n_seq]
+ *   scale      > 0, the factor of the scores (head_dim^-0.5 as a rule)
+ *   out        device [n_seq, heads, head_dim], contiguous; a sequence without a token gets 0
+ *   out_lse    device fp32 [n_seq, heads] or NULL: log of the sum of exp(scaled scores)
+ *   workspace  device scratch of tome_shared_prefix_attention_workspace_bytes, 16-byte aligned;
+ *              needs no initialisation; calls that overlap in time need one each
+ * A length beyond its table counts as the table's; that and a table entry outside
+ * [0, num_blocks), whose tokens read as zeros like in tome_gather_paged_kv, set
+ * TOME_DEV_BLOCK_OUT_OF_RANGE.  Scores and sums in fp32, probabilities rounded to the type of
+ * the values before their product.  n_seq <= 4096, n_groups <= 1024 per call.
+ */
+size_t tome_shared_prefix_attention_workspace_bytes(int64_t n_seq, int64_t n_groups, int64_t heads,
+                                                    int64_t kv_heads, int64_t head_dim);
+int32_t tome_shared_prefix_attention(const void* q, int32_t dtype, int64_t n_seq, int64_t heads,
+                                     int64_t kv_heads, int64_t head_dim, int64_t q_stride,
+                                     const void* k_pool, const void* v_pool, int32_t block_size,
+                                     int32_t num_blocks, const int32_t* prefix_tables,
+                                     const int32_t* prefix_lens, const int32_t* group_starts,
+                                     int64_t n_groups, int32_t prefix_blocks,
+                                     const int32_t* block_tables, const int32_t* lengths,
+                                     int32_t max_blocks, float scale, void* out, float* out_lse,
+                                     void* workspace, size_t workspace_bytes, int32_t* dev_status,
+                                     void* stream);
+
+/*
+ * Clipped policy loss with a k3 KL term, and its gradient with respect to the logits (the
+ * external trainer's part in the reference; windows and layout are those of
+ * tome_dual_logprob_kl).  For an active position with log-prob lp of its target:
+ *   rho = exp(lp - old_logprob),  d = ref_logprob - lp,
+ *   l   = -min(rho a, clamp(rho, 1 - clip_low, 1 + clip_high) a) + kl_coef (exp(d) - d - 1)
+ * and loss = sum of w l with w = 1 / (active positions), or, per_sequence != 0,
+ * 1 / (n_seq * length of the sequence's window).
+ *
+ *   logits     device [n_seq * seq_len, vocab], contiguous, 16-byte aligned, TOME_F32 or TOME_BF16
+ *   targets, old_logprob, ref_logprob   device [n_seq * seq_len]; ref_logprob may be NULL if kl_coef
+ *              is 0 (it is not read then)
+ *   advantages device fp32 [n_seq], or [n_seq * seq_len] with advantage_per_token != 0
+ *   clip_low, clip_high, kl_coef  >= 0 and finite
+ *   grad_scale factor of the gradient (loss scaling, accumulation); the loss does not have it
+ *   out_loss   device fp32 [1]; out_logprob device fp32 [n_seq * seq_len], 0 outside the windows
+ *   out_grad   device, shape and type of logits, contiguous, 16-byte aligned, not overlapping
+ *              them; zeros outside the windows.  NULL: the loss alone, the logits read once
+ *   workspace  device scratch of tome_grpo_policy_loss_workspace_bytes, 16-byte aligned; needs no
+ *              initialisation
+ * Rows outside the windows are never read.  A target outside [0, vocab) makes its row and the
+ * loss NaN and sets TOME_DEV_TARGET_OUT_OF_RANGE.  The sums do not depend on timing.
+ */
+size_t tome_grpo_policy_loss_workspace_bytes(int64_t n_seq, int64_t seq_len);
+int32_t tome_grpo_policy_loss(const void* logits, int32_t dtype, int64_t n_seq, int64_t seq_len,
+                              int64_t vocab, const int32_t* targets, const float* old_logprob,
+                              const float* ref_logprob, const float* advantages,
+                              int32_t advantage_per_token, const int32_t* lengths,
+                              const int32_t* starts, float temperature, float clip_low,
+                              float clip_high, float kl_coef, int32_t per_sequence,
+                              float grad_scale, float* out_loss, float* out_logprob,
+                              void* out_grad, void* workspace, size_t workspace_bytes,
+                              int32_t* dev_status, void* stream);
 
 #ifdef __cplusplus
 }

@@ -11,10 +11,12 @@ import importlib
 
 _OPS = ["BoundCall", "bind_log_softmax", "bind_sample", "bind_selective", "check_device_status",
         "combine_triples", "fused_log_softmax", "gather_paged_kv", "grpo_dual_logprob_kl",
-        "lm_head_logprob", "lm_head_logprob_static", "lm_head_partials",
+        "grpo_policy_loss", "lm_head_logprob", "lm_head_logprob_static", "lm_head_partials",
         "lm_head_workspace_bytes", "local_compute_logprobs", "local_compute_logprobs_host",
-        "ragged_logprobs", "rms_norm", "sample_topk_logprob", "sample_workspace_bytes",
-        "selective_log_softmax", "update_paged_kv"]
+        "qk_norm_rope", "qk_norm_rope_append", "qk_norm_rope_backward", "ragged_logprobs",
+        "rms_norm", "rope_table", "sample_topk_logprob", "sample_workspace_bytes",
+        "selective_log_softmax", "shared_prefix_attention",
+        "shared_prefix_attention_workspace_bytes", "update_paged_kv"]
 _DIST = ["lm_head_logprob_vocab_parallel", "pack_triples", "exchange_triples"]
 _LIB = ["TomeArgumentError", "TomeRuntimeError"]
 

@@ -13,12 +13,14 @@ LIB_PATH = os.path.join(HERE, "libtome_b200.so")
 
 TOME_F32 = 0
 TOME_BF16 = 1
+TOME_F16 = 2
 
 DEV_TARGET_OUT_OF_RANGE = 1
 DEV_TIMEOUT = 2
 DEV_RAGGED_OVERFLOW = 4
 DEV_BLOCK_OUT_OF_RANGE = 8
 DEV_NO_CANDIDATE = 16
+DEV_POSITION_OUT_OF_RANGE = 32
 
 LMHEAD_ROUND_LOGITS_BF16 = 1
 
@@ -66,6 +68,31 @@ SIGNATURES = {
     "tome_update_paged_kv": (c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p,
                                        c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64,
                                        c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "tome_qk_norm_rope": (
+        c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int64, c_void_p, c_void_p, c_void_p,
+                  c_int32, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tome_qk_norm_rope_append": (
+        c_int32, [c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int64, c_void_p, c_void_p, c_void_p,
+                  c_int32, c_void_p, c_float, c_void_p, c_void_p, c_void_p, c_int64, c_int32,
+                  c_int32, c_int32, c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
+    "tome_qk_norm_rope_backward_workspace_bytes": (
+        c_size_t, [c_int32]),
+    "tome_qk_norm_rope_backward": (
+        c_int32, [c_void_p, c_void_p, c_void_p, c_void_p, c_int32, c_int64, c_int32, c_int32, c_int32, c_int64,
+                  c_void_p, c_void_p, c_void_p, c_int32, c_void_p, c_float, c_void_p, c_void_p,
+                  c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "tome_shared_prefix_attention_workspace_bytes": (
+        c_size_t, [c_int64, c_int64, c_int64, c_int64, c_int64]),
+    "tome_shared_prefix_attention": (
+        c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32,
+                  c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
+                  c_int32, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+    "tome_grpo_policy_loss_workspace_bytes": (
+        c_size_t, [c_int64, c_int64]),
+    "tome_grpo_policy_loss": (
+        c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
+                  c_void_p, c_void_p, c_float, c_float, c_float, c_float, c_int32, c_float,
+                  c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
     "tome_combine_triples": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64,
                                        c_int32, c_int64, c_void_p, c_void_p, c_void_p]),
 }

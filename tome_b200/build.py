@@ -17,7 +17,8 @@ CSRC = os.path.join(HERE, "csrc")
 LIB_PATH = os.path.join(HERE, "libtome_b200.so")
 
 SOURCES = ["api.cu", "k1_logprob.cu", "k1_small.cu", "k1_full.cu", "combine.cu", "k2_lmhead.cu",
-           "k4_sample.cu", "k5_paged_kv.cu"]
+           "k4_sample.cu", "k5_paged_kv.cu", "k6_norm_rope.cu", "k7_prefix_attention.cu",
+           "k8_policy_loss.cu"]
 
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a",

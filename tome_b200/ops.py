@@ -19,9 +19,11 @@ from typing import Optional, Tuple
 import torch
 
 from . import _lib
-from ._lib import TOME_BF16, TOME_F32, TomeRuntimeError, check, lib
+from ._lib import TOME_BF16, TOME_F16, TOME_F32, TomeRuntimeError, check, lib
 
 _DTYPES = {torch.float32: TOME_F32, torch.bfloat16: TOME_BF16}
+# what the attention-side operators take besides (qk_norm_rope and the paged attention)
+_MODEL_DTYPES = {**_DTYPES, torch.float16: TOME_F16}
 # sequences tome_dual_logprob_kl / tome_ragged_logprob take per call (the wrappers slice larger batches)
 MAX_SEQ_PER_CALL = 1024
 _status_words: dict = {}
@@ -58,6 +60,8 @@ def check_device_status(device=None) -> None:
         problems.append("a paged-KV block-table entry lies outside the pool")
     if bits & _lib.DEV_NO_CANDIDATE:
         problems.append("sampling met a row without a single logit that is not NaN")
+    if bits & _lib.DEV_POSITION_OUT_OF_RANGE:
+        problems.append("a position lies outside the rotary table")
     if bits & _lib.DEV_TIMEOUT:
         problems.append("a bounded device-side wait ran out (TOME_DEV_TIMEOUT)")
     raise TomeRuntimeError("; ".join(problems) or f"device status {bits}")
@@ -825,3 +829,424 @@ def update_paged_kv(k_new: torch.Tensor, v_new: torch.Tensor, block_tables: torc
             block_size, max_blocks, num_blocks, _status_word(device).data_ptr(), _stream(device))
     _lib.check(status)
     return k_pool, v_pool
+
+
+# ------------------------------------------------------------------ query/key norm + rotation
+def _ints(name: str, t: torch.Tensor, shape, device: torch.device) -> torch.Tensor:
+    """``t`` as a contiguous int32 tensor of ``shape`` on ``device``."""
+    if not isinstance(t, torch.Tensor):
+        t = torch.as_tensor(t)
+    if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
+        raise TypeError(f"{name} must be an integer tensor, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t.to(device=device, dtype=torch.int32).contiguous()
+
+
+def _aligned(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and on a 16-byte boundary (a copy only where it is not)."""
+    t = t if t.is_contiguous() else t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _same(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
+    if t.device != device:
+        _require_cuda(name, t)
+        raise ValueError(f"{name} lives on {t.device}, expected {device}")
+    if t.dtype != dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if tuple(t.shape) != tuple(shape):
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    return t
+
+
+def _out_tensor(name: str, t: Optional[torch.Tensor], shape, dtype: torch.dtype,
+                device: torch.device) -> torch.Tensor:
+    """A caller's output tensor checked, or a fresh one."""
+    if t is None:
+        return torch.empty(shape, dtype=dtype, device=device)
+    _same(name, t, shape, dtype, device)
+    if not t.is_contiguous() or t.data_ptr() % 16:
+        raise ValueError(f"{name} must be contiguous and 16-byte aligned")
+    return t
+
+
+def _span(t: torch.Tensor) -> Tuple[int, int]:
+    """Addresses [begin, end) that a tensor's elements lie in."""
+    if t.numel() == 0:
+        return 0, 0
+    last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
+    return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
+
+
+def _apart(name: str, out: torch.Tensor, **inputs: Optional[torch.Tensor]) -> None:
+    """Refuse an output that shares memory with an input of the same call."""
+    a0, a1 = _span(out)
+    for other, t in inputs.items():
+        if t is not None:
+            b0, b1 = _span(t)
+            if a0 < b1 and b0 < a1:
+                raise ValueError(f"{name} must not overlap {other}")
+
+
+def rope_table(n_positions: int, head_dim: int, base: float = 1000000.0, device=None) -> torch.Tensor:
+    """Rotary table of :func:`qk_norm_rope`: fp32 ``[n_positions, head_dim]``, the cosines of the
+    ``head_dim / 2`` angles ``position * base^(-2 i / head_dim)`` and then their sines.  A model
+    makes it once; the angles are formed in 64 bits, so that far positions keep their accuracy."""
+    if n_positions <= 0 or head_dim <= 0 or head_dim % 2 or not base > 0:
+        raise ValueError(f"n_positions={n_positions} head_dim={head_dim} base={base}")
+    device = torch.device("cuda", torch.cuda.current_device()) if device is None else torch.device(device)
+    half = head_dim // 2
+    freq = float(base) ** (-torch.arange(half, dtype=torch.float64) / half)
+    angle = torch.arange(n_positions, dtype=torch.float64)[:, None] * freq
+    return torch.cat([angle.cos(), angle.sin()], dim=1).to(torch.float32).to(device)
+
+
+def _norm_rope_args(qkv, q_weight, k_weight, cos_sin, positions, heads, kv_heads):
+    """Checked arguments that the three forms share: (rows of qkv, its stride, weights, table,
+    positions, head_dim, dtype code)."""
+    _require_cuda("qkv", qkv)
+    if qkv.dtype not in _MODEL_DTYPES:
+        raise TypeError(f"qkv must be float32, bfloat16 or float16, got {qkv.dtype}")
+    if qkv.dim() < 1:
+        raise ValueError("qkv needs at least one dimension")
+    if heads <= 0 or kv_heads <= 0 or qkv.shape[-1] % (heads + 2 * kv_heads):
+        raise ValueError(f"qkv's last dimension ({qkv.shape[-1]}) is not (heads + 2 kv_heads) = "
+                         f"{heads + 2 * kv_heads} heads wide")
+    width = qkv.shape[-1]
+    dim = width // (heads + 2 * kv_heads)
+    rows, stride = _rows_view(qkv)
+    if rows.data_ptr() % 16 or stride * rows.element_size() % 16:
+        rows = rows.clone(memory_format=torch.contiguous_format)
+        stride = width
+    device = qkv.device
+    qw = _aligned(_same("q_weight", q_weight, (dim,), qkv.dtype, device))
+    kw = _aligned(_same("k_weight", k_weight, (dim,), qkv.dtype, device))
+    if not isinstance(cos_sin, torch.Tensor) or cos_sin.dim() != 2:
+        raise ValueError("cos_sin must be the [n_positions, head_dim] table of rope_table")
+    cs = _aligned(_same("cos_sin", cos_sin, (cos_sin.shape[0], dim), torch.float32, device))
+    pos = _ids32(positions, rows.shape[0], device)
+    return rows, stride, qw, kw, cs, pos, dim, _MODEL_DTYPES[qkv.dtype]
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                 cos_sin: torch.Tensor, positions: torch.Tensor, heads: int, kv_heads: int, *,
+                 eps: float = 1e-6, check: bool = False,
+                 out: Optional[Tuple[torch.Tensor, torch.Tensor]] = None):
+    """Norms of queries and keys for each head and the rotary rotation, in one pass.
+
+    ``qkv`` is the fused projection's output ``[..., (heads + 2 kv_heads) * head_dim]`` (bf16, fp16 or
+    fp32; rows may be views with a pitch), the weights are ``[head_dim]`` in its dtype,
+    ``cos_sin`` is a :func:`rope_table` and ``positions`` holds one integer per token.  Returns
+    ``(q [..., heads, head_dim], k [..., kv_heads, head_dim])``, computed in fp32 and rounded once; the
+    values stay where they are in ``qkv``.  The arithmetic is that of the reference's
+    norm-and-rope kernel (mlx-impl/model.py:105-194).  ``head_dim`` is a multiple of 16 up to 256.
+    A position outside the table gives NaN and a device status (``check=True`` raises).
+    :func:`qk_norm_rope_backward` is its gradient, :func:`qk_norm_rope_append` the form for
+    decoding, which writes keys and values into the paged cache.
+    """
+    rows, stride, qw, kw, cs, pos, dim, code = _norm_rope_args(qkv, q_weight, k_weight, cos_sin,
+                                                               positions, heads, kv_heads)
+    device, n, lead = rows.device, rows.shape[0], tuple(qkv.shape[:-1])
+    q = _out_tensor("out[0] (q)", None if out is None else out[0], lead + (heads, dim), qkv.dtype, device)
+    k = _out_tensor("out[1] (k)", None if out is None else out[1], lead + (kv_heads, dim), qkv.dtype, device)
+    if out is not None:
+        _apart("out[0] (q)", q, qkv=rows, k=k)
+        _apart("out[1] (k)", k, qkv=rows)
+    with _on(device):
+        status = lib.tome_qk_norm_rope(
+            rows.data_ptr(), code, n, heads, kv_heads, dim, stride, qw.data_ptr(), kw.data_ptr(),
+            cs.data_ptr(), cs.shape[0], pos.data_ptr(), float(eps), q.data_ptr(), k.data_ptr(),
+            _status_word(device).data_ptr(), _stream(device))
+    _lib.check(status)
+    if check:
+        check_device_status(device)
+    return q, k
+
+
+def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tensor,
+                        cos_sin: torch.Tensor, positions: torch.Tensor, k_pool: torch.Tensor,
+                        v_pool: torch.Tensor, block_tables: torch.Tensor,
+                        cache_positions: torch.Tensor, *, seq_ids: Optional[torch.Tensor] = None,
+                        eps: float = 1e-6, check: bool = False,
+                        out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """:func:`qk_norm_rope` for serving: returns the queries and appends keys and values to the
+    paged cache (``k_pool``, ``v_pool`` ``[num_blocks, kv_heads, block_size, head_dim]``, IN PLACE).
+
+    Token ``t`` goes to place ``cache_positions[t]`` of sequence ``seq_ids[t]`` (default: token ``t``
+    belongs to sequence ``t``, one token each), that is to block ``block_tables[seq, place //
+    block_size]``; a negative place means the token is not cached.  Unlike
+    :func:`update_paged_kv`, which writes whole blocks from their start, it writes anywhere in
+    a block.  ``positions`` are the rotary positions, which differ from the places where a
+    shared prefix has pages of its own (:func:`shared_prefix_attention`).  A place that the table
+    or the pool does not have is skipped and reported through the device status; two tokens of
+    a call must not name the same place.
+    """
+    for name, t in (("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables)):
+        _require_cuda(name, t)
+    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
+        raise ValueError("k_pool and v_pool must be [num_blocks, H, block_size, D] of one dtype")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError("the pools must be contiguous")
+    num_blocks, kv_heads, block_size, pool_dim = k_pool.shape
+    _require_cuda("qkv", qkv)
+    if pool_dim == 0 or qkv.dim() < 1 or qkv.shape[-1] % pool_dim or \
+            qkv.shape[-1] // pool_dim <= 2 * kv_heads:
+        raise ValueError(f"qkv's last dimension does not hold queries beside {kv_heads} keys and "
+                         f"values of {pool_dim}")
+    heads = qkv.shape[-1] // pool_dim - 2 * kv_heads
+    rows, stride, qw, kw, cs, pos, dim, code = _norm_rope_args(qkv, q_weight, k_weight, cos_sin,
+                                                               positions, heads, kv_heads)
+    device, n, lead = rows.device, rows.shape[0], tuple(qkv.shape[:-1])
+    if k_pool.dtype != qkv.dtype or k_pool.device != device or v_pool.device != device:
+        raise ValueError("the pools must have the dtype and device of qkv")
+    if block_tables.dim() != 2:
+        raise ValueError("block_tables must be [n_seq, max_blocks]")
+    bt = _ints("block_tables", block_tables, block_tables.shape, device)
+    at = _ids32(cache_positions, n, device)
+    sid = None if seq_ids is None else _ids32(seq_ids, n, device)
+    if sid is None and bt.shape[0] != n:
+        raise ValueError(f"without seq_ids there is one token per sequence: {n} tokens, "
+                         f"{bt.shape[0]} sequences")
+    q = _out_tensor("out", out, lead + (heads, dim), qkv.dtype, device)
+    _apart("k_pool", k_pool, qkv=rows, v_pool=v_pool)
+    _apart("v_pool", v_pool, qkv=rows)
+    if out is not None:
+        _apart("out", q, qkv=rows, k_pool=k_pool, v_pool=v_pool)
+    with _on(device):
+        status = lib.tome_qk_norm_rope_append(
+            rows.data_ptr(), code, n, heads, kv_heads, dim, stride, qw.data_ptr(), kw.data_ptr(),
+            cs.data_ptr(), cs.shape[0], pos.data_ptr(), float(eps), _ptr(sid), bt.data_ptr(),
+            at.data_ptr(), bt.shape[0], block_size, bt.shape[1], num_blocks, q.data_ptr(),
+            k_pool.data_ptr(), v_pool.data_ptr(), _status_word(device).data_ptr(), _stream(device))
+    _lib.check(status)
+    if check:
+        check_device_status(device)
+    return q
+
+
+def qk_norm_rope_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, qkv: torch.Tensor,
+                          q_weight: torch.Tensor, k_weight: torch.Tensor, cos_sin: torch.Tensor,
+                          positions: torch.Tensor, *, grad_v: Optional[torch.Tensor] = None,
+                          eps: float = 1e-6, check: bool = False,
+                          out: Optional[torch.Tensor] = None,
+                          workspace: Optional[torch.Tensor] = None):
+    """Gradient of :func:`qk_norm_rope`: ``(grad_qkv, grad_q_weight, grad_k_weight)``.
+
+    ``grad_q`` ``[..., heads, head_dim]`` and ``grad_k`` ``[..., kv_heads, head_dim]`` are the gradients of
+    its outputs, in the dtype of ``qkv``; the other arguments are the forward's, nothing else was
+    kept.  ``grad_qkv`` has the shape and dtype of ``qkv`` (its value part is ``grad_v``, or zeros
+    without it), the weights' gradients are fp32, summed over tokens and heads in an order
+    that depends on the sizes alone.
+    """
+    _require_cuda("grad_q", grad_q)
+    _require_cuda("grad_k", grad_k)
+    _require_cuda("qkv", qkv)
+    if grad_q.dim() < 2 or grad_k.dim() < 2:
+        raise ValueError("grad_q and grad_k must be [..., heads, head_dim]")
+    heads, kv_heads = grad_q.shape[-2], grad_k.shape[-2]
+    rows, stride, qw, kw, cs, pos, dim, code = _norm_rope_args(qkv, q_weight, k_weight, cos_sin,
+                                                               positions, heads, kv_heads)
+    device, n, lead = rows.device, rows.shape[0], tuple(qkv.shape[:-1])
+    gq = _aligned(_same("grad_q", grad_q, lead + (heads, dim), qkv.dtype, device))
+    gk = _aligned(_same("grad_k", grad_k, lead + (kv_heads, dim), qkv.dtype, device))
+    gv = None if grad_v is None else _aligned(_same("grad_v", grad_v, lead + (kv_heads, dim), qkv.dtype, device))
+    grad = _out_tensor("out", out, tuple(qkv.shape), qkv.dtype, device)
+    if out is not None:
+        _apart("out", grad, qkv=rows, grad_q=gq, grad_k=gk, grad_v=gv)
+    nbytes = int(lib.tome_qk_norm_rope_backward_workspace_bytes(dim))
+    ws = _workspace(nbytes, device, workspace)
+    dw = torch.empty((2, dim), dtype=torch.float32, device=device)
+    with _on(device):
+        status = lib.tome_qk_norm_rope_backward(
+            gq.data_ptr(), gk.data_ptr(), _ptr(gv), rows.data_ptr(), code, n, heads, kv_heads, dim,
+            stride, qw.data_ptr(), kw.data_ptr(), cs.data_ptr(), cs.shape[0], pos.data_ptr(), float(eps),
+            grad.data_ptr(), dw[0].data_ptr(), dw[1].data_ptr(), ws.data_ptr(),
+            ws.numel() * ws.element_size(), _status_word(device).data_ptr(), _stream(device))
+    _lib.check(status)
+    if check:
+        check_device_status(device)
+    return grad, dw[0], dw[1]
+
+
+# ------------------------------------------------------------------ paged attention
+def shared_prefix_attention_workspace_bytes(n_seq: int, n_groups: int, heads: int, kv_heads: int,
+                                            head_dim: int) -> int:
+    """Scratch bytes :func:`shared_prefix_attention` needs for a batch of this shape."""
+    return int(lib.tome_shared_prefix_attention_workspace_bytes(n_seq, n_groups, heads, kv_heads, head_dim))
+
+
+def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
+                            prefix_tables: Optional[torch.Tensor],
+                            prefix_lens: Optional[torch.Tensor],
+                            group_starts: Optional[torch.Tensor], block_tables: torch.Tensor,
+                            lengths: torch.Tensor, *, scale: Optional[float] = None,
+                            return_lse: bool = False, check: bool = False,
+                            out: Optional[torch.Tensor] = None,
+                            out_lse: Optional[torch.Tensor] = None,
+                            workspace: Optional[torch.Tensor] = None):
+    """One decode step's attention over the paged cache, each shared prefix read once.
+
+    ``q`` is ``[n_seq, heads, head_dim]`` (bf16 or fp16, head_dim 64 or 128; sequences may be a
+    pitch apart), the pools are ``[num_blocks, kv_heads, block_size, head_dim]`` in its dtype and
+    query head ``h`` reads KV head ``h // (heads / kv_heads)``.  Sequences ``[group_starts[g],
+    group_starts[g + 1])`` attend to the first ``prefix_lens[g]`` tokens of the pages
+    ``prefix_tables[g]``, and each sequence ``b`` to the first ``lengths[b]`` tokens of its own pages
+    ``block_tables[b]`` (the token being decoded among them).  ``prefix_tables``, ``prefix_lens``
+    and ``group_starts`` may all be None: plain paged attention.  Replaces the copies of the
+    prompt's cache and the attention over them (mlx-impl/node.py:529-555, model.py:428).
+
+    Returns ``out [n_seq, heads, head_dim]`` in the dtype of ``q`` and, with ``return_lse`` (or
+    ``out_lse``), the fp32 ``[n_seq, heads]`` log-sum of the exponentials of the scaled scores.
+    ``scale`` defaults to ``head_dim ** -0.5``.  A sequence without a single token gets 0 and -inf.
+    A length beyond its table counts as the table's, and the tokens of a table entry outside the
+    pool read as zeros; both are reported through the device status (``check=True`` raises).
+    ``workspace`` may name a scratch tensor of :func:`shared_prefix_attention_workspace_bytes` bytes,
+    which a decode loop reuses from step to step; calls that overlap in time need one each.
+    """
+    for name, t in (("q", q), ("k_pool", k_pool), ("v_pool", v_pool)):
+        _require_cuda(name, t)
+    if q.dtype not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
+    if q.dim() != 3:
+        raise ValueError("q must be [n_seq, heads, head_dim]")
+    n, heads, dim = q.shape
+    device = q.device
+    if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.shape[3] != dim:
+        raise ValueError("k_pool and v_pool must be [num_blocks, kv_heads, block_size, head_dim]")
+    if k_pool.dtype != q.dtype or v_pool.dtype != q.dtype or k_pool.device != device or \
+            v_pool.device != device:
+        raise ValueError("the pools must have the dtype and device of q")
+    if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
+        raise ValueError("the pools must be contiguous")
+    num_blocks, kv_heads, block_size, _ = k_pool.shape
+    if q.stride(2) == 1 and q.stride(1) == dim and (q.stride(0) >= heads * dim or n <= 1) and \
+            q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0:
+        q_stride = q.stride(0) if n > 1 else heads * dim
+    else:
+        q, q_stride = _aligned(q), heads * dim
+    if not isinstance(block_tables, torch.Tensor) or block_tables.dim() != 2:
+        raise ValueError("block_tables must be [n_seq, max_blocks]")
+    bt = _ints("block_tables", block_tables, (n, block_tables.shape[1]), device)
+    ln = _ints("lengths", lengths, (n,), device)
+    if prefix_tables is None:
+        if prefix_lens is not None or group_starts is not None:
+            raise ValueError("prefix_tables, prefix_lens and group_starts go together")
+        groups, pt, plen, starts = 0, None, None, None
+    else:
+        if prefix_lens is None or group_starts is None:
+            raise ValueError("prefix_tables, prefix_lens and group_starts go together")
+        if not isinstance(prefix_tables, torch.Tensor) or prefix_tables.dim() != 2:
+            raise ValueError("prefix_tables must be [n_groups, prefix_blocks]")
+        groups = prefix_tables.shape[0]
+        pt = _ints("prefix_tables", prefix_tables, prefix_tables.shape, device)
+        plen = _ints("prefix_lens", prefix_lens, (groups,), device)
+        starts = _ints("group_starts", group_starts, (groups + 1,), device)
+    o = _out_tensor("out", out, (n, heads, dim), q.dtype, device)
+    if out is not None:
+        _apart("out", o, q=q, k_pool=k_pool, v_pool=v_pool)
+    if out_lse is not None:
+        _out_tensor("out_lse", out_lse, (n, heads), torch.float32, device)
+        lse, return_lse = out_lse, True
+    else:
+        lse = torch.empty((n, heads), dtype=torch.float32, device=device) if return_lse else None
+    nbytes = shared_prefix_attention_workspace_bytes(n, groups, heads, kv_heads, dim)
+    ws = _workspace(nbytes, device, workspace)
+    with _on(device):
+        status = lib.tome_shared_prefix_attention(
+            q.data_ptr(), _MODEL_DTYPES[q.dtype], n, heads, kv_heads, dim, q_stride, k_pool.data_ptr(),
+            v_pool.data_ptr(), block_size, num_blocks, _ptr(pt), _ptr(plen), _ptr(starts), groups,
+            0 if pt is None else pt.shape[1], bt.data_ptr(), ln.data_ptr(), bt.shape[1],
+            float(dim ** -0.5 if scale is None else scale), o.data_ptr(), _ptr(lse), ws.data_ptr(),
+            ws.numel() * ws.element_size(), _status_word(device).data_ptr(), _stream(device))
+    _lib.check(status)
+    if check:
+        check_device_status(device)
+    return (o, lse) if return_lse else o
+
+
+# ------------------------------------------------------------------ policy loss
+def grpo_policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logprobs: torch.Tensor,
+                     advantages: torch.Tensor, lengths: torch.Tensor, temp: float = 1.0, *,
+                     starts: Optional[torch.Tensor] = None,
+                     ref_logprobs: Optional[torch.Tensor] = None, clip_low: float = 0.2,
+                     clip_high: float = 0.2, kl_coef: float = 0.0, reduction: str = "token",
+                     grad_scale: float = 1.0, return_grad: bool = True, check: bool = False,
+                     out_grad: Optional[torch.Tensor] = None,
+                     workspace: Optional[torch.Tensor] = None):
+    """Clipped policy loss with a k3 KL term and its gradient with respect to the logits.
+
+    ``logits`` is ``[n_seq, seq_len, V]`` (bf16 or fp32); ``ids``, ``old_logprobs`` (the rollout's) and
+    ``ref_logprobs`` (the reference model's, needed where ``kl_coef`` is not 0) are ``[n_seq,
+    seq_len]``; ``advantages`` is ``[n_seq]`` or ``[n_seq, seq_len]``; ``lengths`` and ``starts`` give
+    the window of each sequence, as in :func:`grpo_dual_logprob_kl`.  For a position of a window
+
+        rho = exp(lp - old),  d = ref - lp,
+        l = -min(rho * a, clamp(rho, 1 - clip_low, 1 + clip_high) * a) + kl_coef * (exp(d) - d - 1)
+
+    and the loss is the mean of ``l`` over all positions (``reduction="token"``) or the mean over
+    the sequences of each sequence's mean (``"sequence"``).  Returns ``(loss, logprobs,
+    grad_logits)``: an fp32 scalar, fp32 ``[n_seq, seq_len]`` and a tensor like ``logits``, both zero
+    outside the windows.  The gradient carries the factor ``grad_scale`` (loss scaling, gradient
+    accumulation), the loss does not; continue with ``logits.backward(grad_logits)``, or hand it
+    to the head's own backward.  ``return_grad=False`` gives ``(loss, logprobs)`` from a single
+    read of the logits.  ``out_grad`` names the gradient's tensor, which must not overlap the
+    logits.  The logits are read from HBM once and the gradient is written once; rows outside
+    the windows are not read.  ``temp`` of 0 or None means 1.0.
+    """
+    _require_cuda("logits", logits)
+    if logits.dtype not in _DTYPES:
+        _dtype_code(logits)
+    if logits.dim() != 3:
+        raise ValueError("expected logits of shape [n_seq, seq_len, V]")
+    if reduction not in ("token", "sequence"):
+        raise ValueError(f"reduction must be 'token' or 'sequence', got {reduction!r}")
+    if kl_coef and ref_logprobs is None:
+        raise ValueError("kl_coef needs ref_logprobs")
+    if out_grad is not None and not return_grad:
+        raise ValueError("out_grad without return_grad")
+    temp = float(temp or 1.0)
+    n_seq, seq_len, V = logits.shape
+    device = logits.device
+    lg = _aligned(logits.detach())
+    ids32 = _ids32(ids, n_seq * seq_len, device)
+    len32 = _ids32(lengths, n_seq, device)
+    st32 = None if starts is None else _ids32(starts, n_seq, device)
+
+    def floats(name, t):
+        if not isinstance(t, torch.Tensor) or not t.is_floating_point():
+            raise TypeError(f"{name} must be a floating-point tensor")
+        if t.device != device:
+            raise ValueError(f"{name} lives on {t.device}, expected {device}")
+        return t.detach().to(torch.float32).contiguous()
+
+    old = floats("old_logprobs", old_logprobs)
+    adv = floats("advantages", advantages)
+    ref = floats("ref_logprobs", ref_logprobs) if kl_coef else None
+    for name, t in (("old_logprobs", old), ("ref_logprobs", ref)):
+        if t is not None and tuple(t.shape) != (n_seq, seq_len):
+            raise ValueError(f"{name} must be [n_seq, seq_len] = {(n_seq, seq_len)}, got {tuple(t.shape)}")
+    if tuple(adv.shape) not in ((n_seq,), (n_seq, seq_len)):
+        raise ValueError(f"advantages must be [n_seq] or [n_seq, seq_len], got {tuple(adv.shape)}")
+    grad = None
+    if return_grad:
+        grad = _out_tensor("out_grad", out_grad, (n_seq, seq_len, V), logits.dtype, device)
+        if out_grad is not None:
+            _apart("out_grad", grad, logits=lg)
+    loss = torch.empty((), dtype=torch.float32, device=device)
+    lp = torch.empty((n_seq, seq_len), dtype=torch.float32, device=device)
+    nbytes = int(lib.tome_grpo_policy_loss_workspace_bytes(n_seq, seq_len))
+    ws = _workspace(nbytes, device, workspace)
+    with _on(device):
+        status = lib.tome_grpo_policy_loss(
+            lg.data_ptr(), _DTYPES[lg.dtype], n_seq, seq_len, V, ids32.data_ptr(), old.data_ptr(), _ptr(ref),
+            adv.data_ptr(), int(adv.dim() == 2), len32.data_ptr(), _ptr(st32), temp, float(clip_low),
+            float(clip_high), float(kl_coef), int(reduction == "sequence"), float(grad_scale),
+            loss.data_ptr(), lp.data_ptr(), _ptr(grad), ws.data_ptr(), ws.numel() * ws.element_size(),
+            _status_word(device).data_ptr(), _stream(device))
+    _lib.check(status)
+    if check:
+        check_device_status(device)
+    return (loss, lp, grad) if return_grad else (loss, lp)
