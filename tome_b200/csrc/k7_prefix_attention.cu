@@ -19,7 +19,7 @@
 // pages of any size, rows past the end filled with zeros) into a ring of three stages, one
 // thread issues the tensor-core products S = Q K^T (128 x 64 x D) and O = P V (128 x D x 64),
 // four warps own a row per thread: running maximum and sum, P rounded to the type of V
-// into shared memory, O added up in registers.  S, P and O are double-buffered, so the product
+// into shared memory; O adds up in tensor memory.  S and P are double-buffered, so the products
 // of one tile, the softmax of the next and the loads of the ones behind it overlap.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -38,8 +38,9 @@ constexpr int K7_KEYS = 64;    // keys of a tile
 constexpr int K7_STAGES = 3;
 constexpr int K7_SOFTMAX_WARPS = 4;
 constexpr int K7_MMA_WARP = 4;
-constexpr int K7_COPY_THREADS = 64;
+constexpr int K7_COPY_THREADS = 64;  // a warp fetches half of a tile's keys and values
 constexpr int K7_THREADS = (K7_SOFTMAX_WARPS + 1) * 32 + K7_COPY_THREADS;
+constexpr int K7_SMALL_ROWS = 16;  // pieces of up to this many rows take the warp-level products
 constexpr int K7_MAX_SEQ = 4096;
 constexpr int K7_MAX_GROUPS = 1024;
 
@@ -241,7 +242,8 @@ struct K7Smem {
   static constexpr int O_FULL = P_FULL + 16;               // 2
   static constexpr int Q_EMPTY = O_FULL + 16;              // 2
   static constexpr int TMEM = Q_EMPTY + 16;
-  static constexpr int PLAN = TMEM + 16;
+  static constexpr int WARP_ML = TMEM + 16;                // [4 warps][16 rows] float2
+  static constexpr int PLAN = WARP_ML + 4 * K7_SMALL_ROWS * 8;
   static constexpr int plan_bytes(int n_groups, int n_seq) {
     return 4 * (3 * (n_groups + 1) + n_seq + 1);
   }
@@ -295,6 +297,185 @@ __device__ __forceinline__ void k7_sts128(uint32_t addr, uint4 v) {
                : "memory");
 }
 
+__device__ __forceinline__ void k7_ldmatrix(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void k7_ldmatrix_trans(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// c[16 x 8] += a[16 x 16] b[16 x 8] by one warp
+__device__ __forceinline__ void k7_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                       __nv_bfloat16) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void k7_mma(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1,
+                                       __half) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, "
+      "{%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// A piece of up to 16 rows (a sequence's own tokens, as a rule two to eight rows): each of the
+// four warps takes 16 keys of every tile through warp-level products, with its own running
+// maximum and sum and its sums of p v in registers; they meet at the end of the piece.  The
+// tensor-core path below would compute 128 rows for these few and pass each tile through four
+// barriers; here a tile costs a warp 32 small products and is given back at once.
+template <typename T, int D>
+__device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem, uint32_t base,
+                                               const K7Piece& x, uint32_t& t, uint32_t piece, int warp,
+                                               int lane, float* out_o, float2* out_ml) {
+  using S = K7Smem<D>;
+  const int g = lane >> 2;  // this thread's rows: g and g + 8; its columns: 2 (lane & 3) + {0, 1} of eight
+  bool ok = true;
+  uint32_t qf[D / 16][4];
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
+  float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+  // where this lane points the matrix loads to: row and 16-byte piece of Q, K and V tiles
+  const int q_row = lane & 15, q_c = lane >> 4;
+  const int k_row = warp * 16 + (lane & 7) + ((lane >> 4) << 3), k_c = (lane >> 3) & 1;
+  const int v_row = warp * 16 + (lane & 15), v_c = lane >> 4;
+  for (int32_t j = 0; j < x.n; ++j, ++t) {
+    const uint32_t stage = t % K7_STAGES;
+    if (ok && !mbar_wait(base + S::FULL + stage * 8, (t / K7_STAGES) & 1u)) {
+      k7_raise(p.status, TOME_DEV_TIMEOUT);
+      ok = false;
+    }
+    __syncwarp();
+    if (j == 0) {  // the queries came with the first tile
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int c = 2 * k + q_c;
+        k7_ldmatrix(base + S::Q + (piece & 1u) * S::Q_BYTES + (c >> 3) * (K7_ROWS * 128) + q_row * 128 +
+                        (((c & 7) ^ (q_row & 7)) << 4),
+                    qf[k]);
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(base + S::Q_EMPTY + (piece & 1u) * 8);
+    }
+    const int32_t valid = x.len - (x.tile + j) * K7_KEYS - warp * 16;  // of this warp's 16 keys
+    if (valid > 0) {
+      const uint32_t kt = base + S::KV + stage * S::STAGE, vt = kt + S::KV_BYTES;
+      float s[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int c = 2 * k + k_c;
+        uint32_t b[4];
+        k7_ldmatrix(kt + (c >> 3) * (K7_KEYS * 128) + k_row * 128 + (((c & 7) ^ (k_row & 7)) << 4), b);
+        k7_mma(s[0], qf[k], b[0], b[1], T());
+        k7_mma(s[1], qf[k], b[2], b[3], T());
+      }
+      if (valid < 16) {
+#pragma unroll
+        for (int n = 0; n < 2; ++n)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n * 8 + 2 * (lane & 3) + (e & 1) >= valid) s[n][e] = -INFINITY;
+      }
+      float top[2];
+      bool grow = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * p.c;
+        grow |= g + 8 * r < x.rows && (top[r] > ref[r] + 8.0f || (ref[r] == -INFINITY && top[r] > ref[r]));
+      }
+      if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float next = fmaxf(ref[r], top[r]);
+          const float alpha = next == -INFINITY ? 1.0f : ex2f(ref[r] - next);
+          ref[r] = next;
+          sum[r] *= alpha;
+#pragma unroll
+          for (int i = 0; i < D / 8; ++i) {
+            o[i][2 * r] *= alpha;
+            o[i][2 * r + 1] *= alpha;
+          }
+        }
+      }
+      const float off[2] = {ref[0] == -INFINITY ? 0.0f : -ref[0], ref[1] == -INFINITY ? 0.0f : -ref[1]};
+      uint32_t pf[4];
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          const float a = ex2f(fmaf(s[n][2 * r], p.c, off[r])), b = ex2f(fmaf(s[n][2 * r + 1], p.c, off[r]));
+          sum[r] += a + b;
+          pf[2 * n + r] = k7_pack(a, b, T());
+        }
+#pragma unroll
+      for (int i = 0; i < D / 16; ++i) {
+        const int c = 2 * i + v_c;
+        uint32_t b[4];
+        k7_ldmatrix_trans(vt + (c >> 3) * (K7_KEYS * 128) + v_row * 128 + (((c & 7) ^ (v_row & 7)) << 4), b);
+        k7_mma(o[2 * i], pf, b[0], b[1], T());
+        k7_mma(o[2 * i + 1], pf, b[2], b[3], T());
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(base + S::EMPTY + stage * 8);
+  }
+  // the warps' results meet in the space of P, which is free between pieces: [warp][row][D], pairs
+  // of a row turned by its index so that the eight rows of a store fall on different banks
+  float2* const area = reinterpret_cast<float2*>(smem + S::P);
+  float2* const ml = reinterpret_cast<float2*>(smem + S::WARP_ML);
+#pragma unroll
+  for (int r = 0; r < 2; ++r) {
+    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+    const int row = g + 8 * r;
+    if (row < x.rows) {
+#pragma unroll
+      for (int i = 0; i < D / 8; ++i)
+        area[(warp * K7_SMALL_ROWS + row) * (D / 2) + ((4 * i + (lane & 3)) ^ ((row & 7) << 2))] =
+            make_float2(o[i][2 * r], o[i][2 * r + 1]);
+      if ((lane & 3) == 0) ml[warp * K7_SMALL_ROWS + row] = make_float2(ref[r], sum[r]);
+    }
+  }
+  named_bar_sync(1, K7_SOFTMAX_WARPS * 32);
+  for (int i = warp * 32 + lane; i < x.rows * (D / 2); i += K7_SOFTMAX_WARPS * 32) {
+    const int row = i / (D / 2), f = i - row * (D / 2);
+    float2 w[K7_SOFTMAX_WARPS];
+    float top = -INFINITY;
+#pragma unroll
+    for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
+      w[k] = ml[k * K7_SMALL_ROWS + row];
+      top = fmaxf(top, w[k].x);
+    }
+    float2 v = make_float2(0.0f, 0.0f);
+    float l = 0.0f;
+#pragma unroll
+    for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
+      const float a = w[k].x == -INFINITY ? (w[k].y == 0.0f ? 0.0f : 1.0f) : ex2f(w[k].x - top);
+      const float2 q = area[(k * K7_SMALL_ROWS + row) * (D / 2) + (f ^ ((row & 7) << 2))];
+      v.x = fmaf(a, q.x, v.x);
+      v.y = fmaf(a, q.y, v.y);
+      l = fmaf(a, w[k].y, l);
+    }
+    *reinterpret_cast<float2*>(out_o + row * D + 2 * f) = v;
+    if (f == 0) out_ml[row] = make_float2(top, l);
+  }
+  named_bar_sync(1, K7_SOFTMAX_WARPS * 32);  // P may be written again
+  return ok;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Params p) {
   using S = K7Smem<D>;
@@ -312,13 +493,13 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
   if (threadIdx.x == K7_MMA_WARP * 32) {
     for (int i = 0; i < K7_STAGES; ++i) {
       mbar_init(base + S::FULL + i * 8, K7_COPY_THREADS);
-      mbar_init(base + S::EMPTY + i * 8, 1);
+      mbar_init(base + S::EMPTY + i * 8, K7_SOFTMAX_WARPS);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(base + S::S_FULL + i * 8, 1);
       mbar_init(base + S::P_FULL + i * 8, K7_SOFTMAX_WARPS);
       mbar_init(base + S::O_FULL + i * 8, 1);
-      mbar_init(base + S::Q_EMPTY + i * 8, 1);
+      mbar_init(base + S::Q_EMPTY + i * 8, K7_SOFTMAX_WARPS);
     }
     fence_mbar_init();
   }
@@ -343,7 +524,8 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
     // ------------------------------------------------------------ softmax: thread = row
     const int row = threadIdx.x;
     const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    uint32_t t = 0;
+    // counts of tiles (the ring), of tiles and pieces on the tensor core, of all pieces
+    uint32_t t = 0, u = 0, big_piece = 0, piece = 0;
     bool ok = true;
     // the sequences' places for the joining kernel, dealt over the CTAs
     for (int b = blockIdx.x * K7_SOFTMAX_WARPS * 32 + threadIdx.x; b < p.n_seq;
@@ -364,40 +546,32 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) p.plan[0] = tiles;
 
-    for (int32_t at = first; at < last && ok;) {
+    for (int32_t at = first; at < last && ok; ++piece) {
       const K7Piece x = k7_piece(p, pl, at, last);
       at += x.n;
+      const int64_t slot = static_cast<int64_t>(x.item) + blockIdx.x;
+      const int64_t rows_at = x.prefix ? slot * K7_ROWS : slot * p.ratio;
+      float* const out_o = (x.prefix ? p.prefix_o : p.suffix_o) + rows_at * D;
+      float2* const out_ml = (x.prefix ? p.prefix_ml : p.suffix_ml) + rows_at;
+      if (x.rows <= K7_SMALL_ROWS) {
+        ok = k7_small_piece<T, D>(p, smem, base, x, t, piece, warp, lane, out_o, out_ml);
+        continue;
+      }
       const bool active = warp * 32 < x.rows;  // warps without a row only keep step
-      float o[D];
-#pragma unroll
-      for (int i = 0; i < D; ++i) o[i] = 0.0f;
-      float top = -INFINITY, mc = -INFINITY, sum = 0.0f, alpha = 0.0f;
-      auto add_o = [&](uint32_t tile) {  // o = o * alpha + P V of `tile`
-        if (!mbar_wait(base + S::O_FULL + (tile & 1u) * 8, (tile >> 1) & 1u)) {
-          k7_raise(p.status, TOME_DEV_TIMEOUT);
-          ok = false;
-          return;
-        }
-        __syncwarp();
-        tc_fence_after_sync();
-#pragma unroll
-        for (int h = 0; h < D / 32; ++h) {
-          uint32_t r[32];
-          tmem_ld32(tmem + lanes + 2 * K7_KEYS + (tile & 1u) * D + h * 32, r);
-          tmem_ld_wait_dep(r);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[h * 32 + i] = fmaf(o[h * 32 + i], alpha, __uint_as_float(r[i]));
-        }
-        tc_fence_before_sync();
-      };
-      for (int32_t j = 0; j < x.n && ok; ++j, ++t) {
-        const uint32_t buf = t & 1u;
-        if (!mbar_wait(base + S::S_FULL + buf * 8, (t >> 1) & 1u)) {
+      const uint32_t o_addr = tmem + lanes + 2 * K7_KEYS + (big_piece & 1u) * D;
+      // `ref` is what the exponents are relative to, in the log2 domain.  It follows the row's
+      // maximum only when that has grown by more than 2^8: the sums in tensor memory then
+      // have to be rescaled, which hardly ever happens after the first tiles.
+      float ref = -INFINITY, sum = 0.0f;
+      for (int32_t j = 0; j < x.n && ok; ++j, ++t, ++u) {
+        const uint32_t buf = u & 1u;
+        // S of this tile; the products before it are done too, P V of the tile before last among them, so
+        // that its buffer of P may be written
+        if (!mbar_wait(base + S::S_FULL + buf * 8, (u >> 1) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
           ok = false;
           break;
         }
-        float next_alpha = alpha;
         __syncwarp();
         if (active) {
           tc_fence_after_sync();
@@ -414,75 +588,127 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
               if (i + 32 >= valid) s1[i] = 0xff800000u;
             }
           }
-          float big = top;
+          float big[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-          for (int i = 0; i < 32; ++i) big = fmaxf(big, fmaxf(__uint_as_float(s0[i]), __uint_as_float(s1[i])));
-          // a row that has seen nothing but -inf keeps 0 as its reference: all its p are 0
-          const float mc_new = big == -INFINITY ? 0.0f : big * p.c;
-          next_alpha = top == -INFINITY ? 0.0f : ex2f(mc - mc_new);
-          top = big;
-          mc = mc_new;
-          float l = 0.0f;
+          for (int i = 0; i < 32; ++i)
+            big[i & 3] = fmax3(big[i & 3], __uint_as_float(s0[i]), __uint_as_float(s1[i]));
+          const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * p.c;
+          // (lanes beyond the rows hold whatever the last piece left)
+          const bool grow = row < x.rows && (top > ref + 8.0f || (j == 0 && top > ref));
+          if (__any_sync(0xffffffffu, grow)) {
+            const float next = grow ? top : ref;
+            const float alpha = next == -INFINITY ? 1.0f : ex2f(ref - next);
+            sum *= alpha;
+            ref = next;
+            if (j > 0) {
+              if (!mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u)) {
+                k7_raise(p.status, TOME_DEV_TIMEOUT);
+                ok = false;
+              }
+              __syncwarp();
+              tc_fence_after_sync();
+#pragma unroll 1
+              for (int h = 0; h < D; h += 32) {
+                uint32_t r[32];
+                tmem_ld32(o_addr + h, r);
+                tmem_ld_wait_dep(r);
+#pragma unroll
+                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
+                tmem_st32(o_addr + h, r);
+              }
+              tmem_st_wait();
+            }
+          }
+          // a row that has seen nothing but -inf takes 0 as its reference: all its p are 0
+          const float off = ref == -INFINITY ? 0.0f : -ref;
+          const float2 c2 = make_float2(p.c, p.c), off2 = make_float2(off, off);
+          float2 la = make_float2(0.0f, 0.0f), lb = la;
           const uint32_t prow = base + S::P + buf * S::P_BYTES + row * 128;
 #pragma unroll
           for (int h = 0; h < 8; ++h) {  // eight keys: one 16-byte piece of P
-            float e[8];
+            float2 e[4];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-              const uint32_t w = h < 4 ? s0[(h & 3) * 8 + i] : s1[(h & 3) * 8 + i];
-              e[i] = ex2f(fmaf(__uint_as_float(w), p.c, -mc));
-              l += e[i];
+            for (int i = 0; i < 4; ++i) {
+              const int w = (h & 3) * 8 + 2 * i;
+              e[i] = h < 4 ? make_float2(__uint_as_float(s0[w]), __uint_as_float(s0[w + 1]))
+                           : make_float2(__uint_as_float(s1[w]), __uint_as_float(s1[w + 1]));
+              e[i] = __ffma2_rn(e[i], c2, off2);
+              e[i].x = ex2f(e[i].x);
+              e[i].y = ex2f(e[i].y);
             }
+            la = __fadd2_rn(la, __fadd2_rn(e[0], e[1]));
+            lb = __fadd2_rn(lb, __fadd2_rn(e[2], e[3]));
             k7_sts128(prow + ((h ^ (row & 7)) << 4),
-                      make_uint4(k7_pack(e[0], e[1], T()), k7_pack(e[2], e[3], T()),
-                                 k7_pack(e[4], e[5], T()), k7_pack(e[6], e[7], T())));
+                      make_uint4(k7_pack(e[0].x, e[0].y, T()), k7_pack(e[1].x, e[1].y, T()),
+                                 k7_pack(e[2].x, e[2].y, T()), k7_pack(e[3].x, e[3].y, T())));
           }
-          sum = fmaf(sum, next_alpha, l);
+          sum += (la.x + la.y) + (lb.x + lb.y);
           fence_proxy_async();
           tc_fence_before_sync();
         }
         __syncwarp();
         if (lane == 0) mbar_arrive(base + S::P_FULL + buf * 8);
-        if (active && j > 0) add_o(t - 1);
-        alpha = next_alpha;
       }
-      if (active && ok) add_o(t - 1);
-      if (ok && row < x.rows) {
-        const int64_t slot = static_cast<int64_t>(x.item) + blockIdx.x;
-        const int64_t at_row = x.prefix ? slot * K7_ROWS + row : slot * p.ratio + row;
-        float* dst = (x.prefix ? p.prefix_o : p.suffix_o) + at_row * D;
+      ++big_piece;
+      // (warps without a row wait too: what follows may write where the products read P)
+      if (ok && !mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u)) {
+        k7_raise(p.status, TOME_DEV_TIMEOUT);
+        ok = false;
+      }
+      if (!active || !ok) continue;
+      __syncwarp();
+      tc_fence_after_sync();
+      float* dst = out_o + row * D;
+#pragma unroll 1
+      for (int h = 0; h < D; h += 32) {
+        uint32_t r[32];
+        tmem_ld32(o_addr + h, r);
+        tmem_ld_wait_dep(r);
+        if (row < x.rows) {
 #pragma unroll
-        for (int i = 0; i < D; i += 4)
-          *reinterpret_cast<float4*>(dst + i) = make_float4(o[i], o[i + 1], o[i + 2], o[i + 3]);
-        (x.prefix ? p.prefix_ml : p.suffix_ml)[at_row] = make_float2(mc, sum);
+          for (int i = 0; i < 32; i += 4)
+            stg128(dst + h + i, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]));
+        }
       }
+      tc_fence_before_sync();
+      if (row < x.rows) out_ml[row] = make_float2(ref, sum);
     }
   } else if (warp == K7_MMA_WARP) {
     // ------------------------------------------------------------ tensor-core products
     if (lane == 0) {
-      uint32_t t = 0, piece = 0;
-      bool ok = true;
-      auto multiply_pv = [&](uint32_t tile) {  // O = P V of `tile`, and its stage is free
-        if (!mbar_wait(base + S::P_FULL + (tile & 1u) * 8, (tile >> 1) & 1u)) {
+      // counts as above; the product P V of a tile is issued after Q K of the next one
+      uint32_t t = 0, u = 0, big_piece = 0, piece = 0;
+      bool ok = true, pending = false, pending_add = false;
+      uint32_t pending_stage = 0, pending_o = 0;
+      auto multiply_pv = [&]() {  // O (+)= P V of tile u - 1
+        pending = false;
+        const uint32_t buf = (u - 1) & 1u;
+        if (!mbar_wait(base + S::P_FULL + buf * 8, ((u - 1) >> 1) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
           ok = false;
           return;
         }
         tc_fence_after_sync();
-        const uint32_t stage = tile % K7_STAGES;
-        const uint64_t a = k7_desc_k(base + S::P + (tile & 1u) * S::P_BYTES);
-        const uint64_t b = k7_desc_mn(base + S::KV + stage * S::STAGE + S::KV_BYTES, K7_KEYS * 128);
+        const uint64_t a = k7_desc_k(base + S::P + buf * S::P_BYTES);
+        const uint64_t b = k7_desc_mn(base + S::KV + pending_stage * S::STAGE + S::KV_BYTES, K7_KEYS * 128);
 #pragma unroll
         for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 32 bytes of a P row, 16 rows of V
-          umma_bf16_ss(tmem + 2 * K7_KEYS + (tile & 1u) * D, a + 2 * k, b + (2048 >> 4) * k,
-                       k7_idesc<T>(D, true), k != 0);
-        umma_commit(base + S::O_FULL + (tile & 1u) * 8);
-        umma_commit(base + S::EMPTY + stage * 8);
+          umma_bf16_ss(tmem + 2 * K7_KEYS + pending_o * D, a + 2 * k, b + (2048 >> 4) * k,
+                       k7_idesc<T>(D, true), pending_add || k != 0);
+        // a stage is given back by four arrivals (of four warps, where those do the products)
+        for (int i = 1; i < K7_SOFTMAX_WARPS; ++i) mbar_arrive(base + S::EMPTY + pending_stage * 8);
+        umma_commit(base + S::EMPTY + pending_stage * 8);
+        umma_commit(base + S::O_FULL + buf * 8);
       };
       for (int32_t at = first; at < last && ok; ++piece) {
-        const int32_t n = k7_piece(p, pl, at, last).n;
-        at += n;
-        for (int32_t j = 0; j < n && ok; ++j, ++t) {
+        const K7Piece x = k7_piece(p, pl, at, last);
+        at += x.n;
+        if (x.rows <= K7_SMALL_ROWS) {
+          if (pending) multiply_pv();
+          t += x.n;
+          continue;
+        }
+        for (int32_t j = 0; j < x.n && ok; ++j, ++t) {
           const uint32_t stage = t % K7_STAGES;
           if (!mbar_wait(base + S::FULL + stage * 8, (t / K7_STAGES) & 1u)) {
             k7_raise(p.status, TOME_DEV_TIMEOUT);
@@ -495,39 +721,67 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           for (int k = 0; k < D / 16; ++k) {
             const uint64_t a = k7_desc_k(base + S::Q + (piece & 1u) * S::Q_BYTES + (k / 4) * (K7_ROWS * 128)) + 2 * (k % 4);
             const uint64_t b = k7_desc_k(base + S::KV + stage * S::STAGE + (k / 4) * (K7_KEYS * 128)) + 2 * (k % 4);
-            umma_bf16_ss(tmem + (t & 1u) * K7_KEYS, a, b, k7_idesc<T>(K7_KEYS, false), k != 0);
+            umma_bf16_ss(tmem + (u & 1u) * K7_KEYS, a, b, k7_idesc<T>(K7_KEYS, false), k != 0);
           }
-          umma_commit(base + S::S_FULL + (t & 1u) * 8);
-          if (j == n - 1) umma_commit(base + S::Q_EMPTY + (piece & 1u) * 8);
-          if (t > 0) multiply_pv(t - 1);
+          umma_commit(base + S::S_FULL + (u & 1u) * 8);
+          if (j == x.n - 1) {
+            for (int i = 1; i < K7_SOFTMAX_WARPS; ++i) mbar_arrive(base + S::Q_EMPTY + (piece & 1u) * 8);
+            umma_commit(base + S::Q_EMPTY + (piece & 1u) * 8);
+          }
+          if (pending) multiply_pv();
+          pending = true;
+          pending_add = j > 0;
+          pending_stage = stage;
+          pending_o = big_piece & 1u;
+          ++u;
         }
+        ++big_piece;
       }
-      if (ok && t > 0) multiply_pv(t - 1);
+      if (ok && pending) multiply_pv();
       // nothing may still be under way when the block leaves
-      if (ok && t > 0 && !mbar_wait(base + S::EMPTY + ((t - 1) % K7_STAGES) * 8, ((t - 1) / K7_STAGES) & 1u))
+      if (ok && u > 0 && !mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u))
         k7_raise(p.status, TOME_DEV_TIMEOUT);
     }
     __syncwarp();
   } else {
     // ------------------------------------------------------------ copies
-    constexpr int PIECES = D / 8;                        // 16-byte pieces of a row
-    constexpr int STEP = K7_COPY_THREADS / PIECES;       // rows per sweep
-    constexpr int SWEEPS = K7_KEYS / STEP;
-    const int ct = threadIdx.x - (K7_MMA_WARP + 1) * 32;
-    const int c = ct % PIECES, r0 = ct / PIECES;
-    const T* kp = reinterpret_cast<const T*>(p.k_pool) + c * 8;
-    const T* vp = reinterpret_cast<const T*>(p.v_pool) + c * 8;
+    constexpr int PIECES = D / 8;                  // 16-byte pieces of a row
+    constexpr int AT_ONCE = 32 / PIECES;           // rows that a warp copies per step
+    constexpr int STEPS = 32 / AT_ONCE;            // a warp has 32 of the 64 keys
+    const int cw = warp - (K7_MMA_WARP + 1);
+    const int c = lane % PIECES, sub = lane / PIECES;
+    const int my_row = cw * 32;
+    const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
+    const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
+    const uint32_t area = base + S::KV + (c >> 3) * (K7_KEYS * 128);
+    // Row of the pool (heads and blocks flattened) of key (tile * 64 + my_row + lane), or -1.
+    auto find_row = [&](const K7Piece& x, int32_t tile) -> int32_t {
+      const int32_t key = tile * K7_KEYS + my_row + lane;
+      if (key >= x.len) return -1;
+      const int32_t blk = static_cast<int32_t>((static_cast<uint64_t>(key) * p.div_magic) >> p.div_shift);
+      const int32_t page = __ldg(x.table + blk);
+      if (page < 0 || page >= p.num_blocks) {
+        k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);  // reads as zeros, as gather does
+        return -1;
+      }
+      return (page * p.kv_heads + x.kv_head) * p.block_size + (key - blk * p.block_size);
+    };
     uint32_t t = 0, piece = 0;
     bool ok = true;
-    for (int32_t at = first; at < last && ok; ++piece) {
-      const K7Piece x = k7_piece(p, pl, at, last);
-      at += x.n;
+    int32_t at = first;
+    K7Piece x;
+    int32_t pool_row = -1;
+    if (at < last) {
+      x = k7_piece(p, pl, at, last);
+      pool_row = find_row(x, x.tile);
+    }
+    while (at < last && ok) {
       if (piece >= 2 && !mbar_wait(base + S::Q_EMPTY + (piece & 1u) * 8, ((piece >> 1) - 1) & 1u)) {
         k7_raise(p.status, TOME_DEV_TIMEOUT);
         ok = false;
         break;
       }
-      for (int i = r0; i < x.rows; i += STEP) {
+      for (int i = cw * AT_ONCE + sub; i < x.rows; i += 2 * AT_ONCE) {
         const int32_t row = x.row0 + i, s = row / p.ratio;
         const T* src = reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
                        static_cast<int64_t>(x.kv_head * p.ratio + (row - s * p.ratio)) * D + c * 8;
@@ -535,40 +789,40 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
                       (((c & 7) ^ (i & 7)) << 4),
                   src, true);
       }
-      for (int32_t j = 0; j < x.n && ok; ++j, ++t) {
+      K7Piece next = x;
+      const int32_t end = at + x.n;
+      for (int32_t j = 0; j < x.n; ++j, ++t) {
         const uint32_t stage = t % K7_STAGES;
-        // where the keys are, ahead of the wait for the stage
-        int64_t src[SWEEPS];
-#pragma unroll
-        for (int i = 0; i < SWEEPS; ++i) {
-          const int32_t key = (x.tile + j) * K7_KEYS + r0 + i * STEP;
-          src[i] = -1;
-          if (key < x.len) {
-            const int32_t blk = static_cast<int32_t>((static_cast<uint64_t>(key) * p.div_magic) >> p.div_shift);
-            const int32_t page = __ldg(x.table + blk);
-            if (page >= 0 && page < p.num_blocks)
-              src[i] = ((static_cast<int64_t>(page) * p.kv_heads + x.kv_head) * p.block_size +
-                        (key - blk * p.block_size)) * D;
-            else
-              k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);  // reads as zeros, as gather does
-          }
+        // the next tile's rows are asked for before this one's copies go out
+        int32_t next_row = -1;
+        if (j + 1 < x.n) {
+          next_row = find_row(x, x.tile + j + 1);
+        } else if (end < last) {
+          next = k7_piece(p, pl, end, last);
+          next_row = find_row(next, next.tile);
         }
         if (t >= K7_STAGES && !mbar_wait(base + S::EMPTY + stage * 8, (t / K7_STAGES - 1) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
           ok = false;
           break;
         }
-        const uint32_t dst = base + S::KV + stage * S::STAGE + (c >> 3) * (K7_KEYS * 128);
+        __syncwarp();
+        const uint32_t dst = area + stage * S::STAGE;
 #pragma unroll
-        for (int i = 0; i < SWEEPS; ++i) {
-          const int r = r0 + i * STEP;
-          const uint32_t d = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-          const int64_t off = src[i] < 0 ? 0 : src[i];
-          k7_copy16(d, kp + off, src[i] >= 0);
-          k7_copy16(d + S::KV_BYTES, vp + off, src[i] >= 0);
+        for (int i = 0; i < STEPS; ++i) {
+          const int r = my_row + i * AT_ONCE + sub;
+          const int32_t from = __shfl_sync(0xffffffffu, pool_row, i * AT_ONCE + sub);
+          const int64_t off = static_cast<int64_t>(max(from, 0)) * D;
+          const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          k7_copy16(to, k_pool + off, from >= 0);
+          k7_copy16(to + S::KV_BYTES, v_pool + off, from >= 0);
         }
         k7_copies_arrive(base + S::FULL + stage * 8);
+        pool_row = next_row;
       }
+      at = end;
+      x = next;
+      ++piece;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
   }
@@ -780,6 +1034,8 @@ extern "C" int32_t tome_shared_prefix_attention(
       static_cast<int64_t>(max_blocks) * block_size > 0x3fffffff ||
       row_blocks * kv_heads * key_tiles + n_seq * kv_heads * seq_tiles > 0x3fffffff)
     return fail(TOME_ERR_TOO_LARGE, "the tables name too many keys for one call");
+  if (static_cast<int64_t>(num_blocks) * kv_heads > 0x7fffffff / block_size)
+    return fail(TOME_ERR_TOO_LARGE, "the pool has more than 2^31 - 1 rows");
   DeviceInfo info;
   st = current_device_info(&info);
   if (st != TOME_OK) return st;

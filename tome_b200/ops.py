@@ -834,6 +834,9 @@ def update_paged_kv(k_new: torch.Tensor, v_new: torch.Tensor, block_tables: torc
 # ------------------------------------------------------------------ query/key norm + rotation
 def _ints(name: str, t: torch.Tensor, shape, device: torch.device) -> torch.Tensor:
     """``t`` as a contiguous int32 tensor of ``shape`` on ``device``."""
+    if isinstance(t, torch.Tensor) and t.dtype is torch.int32 and t.shape == shape and \
+            t.device == device and t.is_contiguous():
+        return t
     if not isinstance(t, torch.Tensor):
         t = torch.as_tensor(t)
     if t.is_floating_point() or t.is_complex() or t.dtype == torch.bool:
@@ -843,6 +846,14 @@ def _ints(name: str, t: torch.Tensor, shape, device: torch.device) -> torch.Tens
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
+def _index(ids: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:
+    """:func:`_ids32` for a tensor of any shape, without a call where nothing is to be done."""
+    if isinstance(ids, torch.Tensor) and ids.dtype is torch.int32 and ids.device == device and \
+            ids.numel() == n and ids.is_contiguous():
+        return ids
+    return _ids32(ids, n, device)
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """``t`` contiguous and on a 16-byte boundary (a copy only where it is not)."""
     t = t if t.is_contiguous() else t.contiguous()
@@ -850,6 +861,8 @@ def _aligned(t: torch.Tensor) -> torch.Tensor:
 
 
 def _same(name: str, t: torch.Tensor, shape, dtype: torch.dtype, device: torch.device) -> torch.Tensor:
+    if isinstance(t, torch.Tensor) and t.dtype is dtype and t.shape == shape and t.device == device:
+        return t
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
     if t.device != device:
@@ -877,6 +890,8 @@ def _span(t: torch.Tensor) -> Tuple[int, int]:
     """Addresses [begin, end) that a tensor's elements lie in."""
     if t.numel() == 0:
         return 0, 0
+    if t.is_contiguous():
+        return t.data_ptr(), t.data_ptr() + t.numel() * t.element_size()
     last = sum((n - 1) * st for n, st in zip(t.shape, t.stride()))
     return t.data_ptr(), t.data_ptr() + (last + 1) * t.element_size()
 
@@ -904,6 +919,20 @@ def rope_table(n_positions: int, head_dim: int, base: float = 1000000.0, device=
     return torch.cat([angle.cos(), angle.sin()], dim=1).to(torch.float32).to(device)
 
 
+_query_bytes: dict = {}
+
+
+def _cached_bytes(query, *sizes) -> int:
+    """Answer of a workspace query of the library (it depends on the sizes alone), remembered."""
+    key = (query.__name__, *sizes)
+    n = _query_bytes.get(key)
+    if n is None:
+        if len(_query_bytes) >= 4096:
+            _query_bytes.clear()
+        n = _query_bytes[key] = int(query(*sizes))
+    return n
+
+
 def _norm_rope_args(qkv, q_weight, k_weight, cos_sin, positions, heads, kv_heads):
     """Checked arguments that the three forms share: (rows of qkv, its stride, weights, table,
     positions, head_dim, dtype code)."""
@@ -927,7 +956,7 @@ def _norm_rope_args(qkv, q_weight, k_weight, cos_sin, positions, heads, kv_heads
     if not isinstance(cos_sin, torch.Tensor) or cos_sin.dim() != 2:
         raise ValueError("cos_sin must be the [n_positions, head_dim] table of rope_table")
     cs = _aligned(_same("cos_sin", cos_sin, (cos_sin.shape[0], dim), torch.float32, device))
-    pos = _ids32(positions, rows.shape[0], device)
+    pos = _index(positions, rows.shape[0], device)
     return rows, stride, qw, kw, cs, pos, dim, _MODEL_DTYPES[qkv.dtype]
 
 
@@ -1005,14 +1034,16 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
     if block_tables.dim() != 2:
         raise ValueError("block_tables must be [n_seq, max_blocks]")
     bt = _ints("block_tables", block_tables, block_tables.shape, device)
-    at = _ids32(cache_positions, n, device)
-    sid = None if seq_ids is None else _ids32(seq_ids, n, device)
+    at = _index(cache_positions, n, device)
+    sid = None if seq_ids is None else _index(seq_ids, n, device)
     if sid is None and bt.shape[0] != n:
         raise ValueError(f"without seq_ids there is one token per sequence: {n} tokens, "
                          f"{bt.shape[0]} sequences")
     q = _out_tensor("out", out, lead + (heads, dim), qkv.dtype, device)
-    _apart("k_pool", k_pool, qkv=rows, v_pool=v_pool)
-    _apart("v_pool", v_pool, qkv=rows)
+    kp, vp = k_pool.data_ptr(), v_pool.data_ptr()
+    pool_bytes = k_pool.numel() * k_pool.element_size()
+    if kp < vp + pool_bytes and vp < kp + pool_bytes and pool_bytes:
+        raise ValueError("k_pool must not overlap v_pool")
     if out is not None:
         _apart("out", q, qkv=rows, k_pool=k_pool, v_pool=v_pool)
     with _on(device):
@@ -1020,7 +1051,7 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
             rows.data_ptr(), code, n, heads, kv_heads, dim, stride, qw.data_ptr(), kw.data_ptr(),
             cs.data_ptr(), cs.shape[0], pos.data_ptr(), float(eps), _ptr(sid), bt.data_ptr(),
             at.data_ptr(), bt.shape[0], block_size, bt.shape[1], num_blocks, q.data_ptr(),
-            k_pool.data_ptr(), v_pool.data_ptr(), _status_word(device).data_ptr(), _stream(device))
+            kp, vp, _status_word(device).data_ptr(), _stream(device))
     _lib.check(status)
     if check:
         check_device_status(device)
@@ -1056,26 +1087,28 @@ def qk_norm_rope_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, qkv: torch
     grad = _out_tensor("out", out, tuple(qkv.shape), qkv.dtype, device)
     if out is not None:
         _apart("out", grad, qkv=rows, grad_q=gq, grad_k=gk, grad_v=gv)
-    nbytes = int(lib.tome_qk_norm_rope_backward_workspace_bytes(dim))
+    nbytes = _cached_bytes(lib.tome_qk_norm_rope_backward_workspace_bytes, dim)
     ws = _workspace(nbytes, device, workspace)
-    dw = torch.empty((2, dim), dtype=torch.float32, device=device)
+    dqw = torch.empty(dim, dtype=torch.float32, device=device)
+    dkw = torch.empty(dim, dtype=torch.float32, device=device)
     with _on(device):
         status = lib.tome_qk_norm_rope_backward(
             gq.data_ptr(), gk.data_ptr(), _ptr(gv), rows.data_ptr(), code, n, heads, kv_heads, dim,
             stride, qw.data_ptr(), kw.data_ptr(), cs.data_ptr(), cs.shape[0], pos.data_ptr(), float(eps),
-            grad.data_ptr(), dw[0].data_ptr(), dw[1].data_ptr(), ws.data_ptr(),
+            grad.data_ptr(), dqw.data_ptr(), dkw.data_ptr(), ws.data_ptr(),
             ws.numel() * ws.element_size(), _status_word(device).data_ptr(), _stream(device))
     _lib.check(status)
     if check:
         check_device_status(device)
-    return grad, dw[0], dw[1]
+    return grad, dqw, dkw
 
 
 # ------------------------------------------------------------------ paged attention
 def shared_prefix_attention_workspace_bytes(n_seq: int, n_groups: int, heads: int, kv_heads: int,
                                             head_dim: int) -> int:
     """Scratch bytes :func:`shared_prefix_attention` needs for a batch of this shape."""
-    return int(lib.tome_shared_prefix_attention_workspace_bytes(n_seq, n_groups, heads, kv_heads, head_dim))
+    return _cached_bytes(lib.tome_shared_prefix_attention_workspace_bytes, n_seq, n_groups, heads,
+                         kv_heads, head_dim)
 
 
 def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch.Tensor,
@@ -1211,9 +1244,9 @@ def grpo_policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logprobs: torc
     n_seq, seq_len, V = logits.shape
     device = logits.device
     lg = _aligned(logits.detach())
-    ids32 = _ids32(ids, n_seq * seq_len, device)
-    len32 = _ids32(lengths, n_seq, device)
-    st32 = None if starts is None else _ids32(starts, n_seq, device)
+    ids32 = _index(ids, n_seq * seq_len, device)
+    len32 = _index(lengths, n_seq, device)
+    st32 = None if starts is None else _index(starts, n_seq, device)
 
     def floats(name, t):
         if not isinstance(t, torch.Tensor) or not t.is_floating_point():
@@ -1237,7 +1270,7 @@ def grpo_policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logprobs: torc
             _apart("out_grad", grad, logits=lg)
     loss = torch.empty((), dtype=torch.float32, device=device)
     lp = torch.empty((n_seq, seq_len), dtype=torch.float32, device=device)
-    nbytes = int(lib.tome_grpo_policy_loss_workspace_bytes(n_seq, seq_len))
+    nbytes = _cached_bytes(lib.tome_grpo_policy_loss_workspace_bytes, n_seq, seq_len)
     ws = _workspace(nbytes, device, workspace)
     with _on(device):
         status = lib.tome_grpo_policy_loss(
