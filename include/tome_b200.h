@@ -415,7 +415,7 @@ int32_t tome_qk_norm_rope_backward(const void* grad_q, const void* grad_k, const
  * A length beyond its table counts as the table's; that and a table entry outside
  * [0, num_blocks), whose tokens read as zeros like in tome_gather_paged_kv, set
  * TOME_DEV_BLOCK_OUT_OF_RANGE.  Scores and sums in fp32, probabilities rounded to the type of
- * the values before their product.  n_seq <= 4096, n_groups <= 1024 per call.
+ * the values before their product.  n_seq <= 2048, n_groups <= 512 per call.
  */
 size_t tome_shared_prefix_attention_workspace_bytes(int64_t n_seq, int64_t n_groups, int64_t heads,
                                                     int64_t kv_heads, int64_t head_dim);

@@ -9,17 +9,18 @@
 //
 // Work.  An item is (KV head, up to 128 query rows that read the same keys): the rows of a
 // group against its prefix, or of one sequence against its suffix.  Items are cut into tiles of
-// 64 keys, all tiles are laid end to end and every CTA takes an equal run of them, whatever the
-// lengths: the split follows from the lengths on the device alone.  A CTA's part of an item is a
+// 64 keys, weighed by what they cost (an item K7_ITEM_COST, a tile K7_SMALL_COST or K7_BIG_COST, see
+// there) and laid end to end; every CTA takes an equal run of the whole, whatever the lengths: the
+// split follows from the lengths on the device alone.  A CTA's part of an item is a
 // piece; it leaves (sum of p v, row maximum, row sum) in the workspace, and a second kernel
 // joins the pieces of a row.  A row's pieces lie at (item index + CTA index), which no two pieces
 // share since at least one of the two grows from piece to piece.
 //
 // Pipeline of a CTA (one per SM): two warps copy keys and values (16-byte asynchronous copies:
-// pages of any size, rows past the end filled with zeros) into a ring of three stages, one
+// pages of any size, rows past the end filled with zeros) into a ring of four stages, one
 // thread issues the tensor-core products S = Q K^T (128 x 64 x D) and O = P V (128 x D x 64),
 // four warps own a row per thread: running maximum and sum, P rounded to the type of V
-// into shared memory; O adds up in tensor memory.  S and P are double-buffered, so the products
+// into shared memory; O adds up in tensor memory.  S is double-buffered, so the products
 // of one tile, the softmax of the next and the loads of the ones behind it overlap.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -35,14 +36,22 @@ namespace tome {
 
 constexpr int K7_ROWS = 128;   // query rows of an item (TMEM lanes)
 constexpr int K7_KEYS = 64;    // keys of a tile
-constexpr int K7_STAGES = 3;
+constexpr int K7_STAGES = 4;
 constexpr int K7_SOFTMAX_WARPS = 4;
 constexpr int K7_MMA_WARP = 4;
 constexpr int K7_COPY_THREADS = 64;  // a warp fetches half of a tile's keys and values
 constexpr int K7_THREADS = (K7_SOFTMAX_WARPS + 1) * 32 + K7_COPY_THREADS;
 constexpr int K7_SMALL_ROWS = 16;  // pieces of up to this many rows take the warp-level products
-constexpr int K7_MAX_SEQ = 4096;
-constexpr int K7_MAX_GROUPS = 1024;
+// Costs, in thirds of a tile of few rows: a tile of up to 16 rows, one of more, and what a piece
+// costs besides its tiles (the ring runs dry while the queries come, the warps' results meet).
+constexpr int K7_SMALL_COST = 3;
+constexpr int K7_BIG_COST = 4;
+constexpr int K7_ITEM_COST = 4;
+// Cards of pieces in flight.  One is written over four pieces later; the copying warps are at most
+// two pieces ahead of a Q buffer's release, and that comes after the softmax warps took the card.
+constexpr int K7_CARDS = 4;
+constexpr int K7_MAX_SEQ = 2048;
+constexpr int K7_MAX_GROUPS = 512;
 
 struct K7Params {
   const void* q;              // [n_seq, heads, D], sequence stride q_stride
@@ -60,7 +69,7 @@ struct K7Params {
   float c;                    // scale * log2(e)
   int32_t ctas;               // CTAs of the main kernel
   // workspace
-  int32_t* plan;              // [0]: tiles in all; then int4 [n_seq] and int2 [n_seq], see K7Plan
+  int32_t* plan;              // [0]: the cost of all items; then two int4 [n_seq], see the kernel
   float* prefix_o;            // [prefix slots, 128, D]
   float2* prefix_ml;          // [prefix slots, 128] (maximum * c, sum)
   float* suffix_o;            // [suffix slots, ratio, D]
@@ -84,11 +93,23 @@ __device__ __forceinline__ int32_t k7_length(const K7Params& p, int32_t len, int
 struct K7Plan {
   int32_t* group;   // [n_groups + 1] first sequence of each group (clamped, not decreasing)
   int32_t* block;   // [n_groups + 1] row blocks (of 128 rows) before each group
-  int32_t* prefix;  // [n_groups + 1] prefix tiles before each group, all KV heads
-  int32_t* suffix;  // [n_seq + 1] suffix tiles before each sequence, all KV heads
+  int32_t* prefix;  // [n_groups + 1] cost of the prefix items before each group
+  int32_t* suffix;  // [n_seq + 1] cost of the suffix items before each sequence
 };
 
 __device__ __forceinline__ int32_t k7_tiles(int32_t len) { return (len + K7_KEYS - 1) / K7_KEYS; }
+
+// Cost of a tile of an item whose rows number `rows`, and of an item; tiles that lie before the
+// offset `cost` of an item.
+__device__ __forceinline__ int32_t k7_tile_cost(int32_t rows) {
+  return rows <= K7_SMALL_ROWS ? K7_SMALL_COST : K7_BIG_COST;
+}
+__device__ __forceinline__ int32_t k7_item_cost(int32_t tiles, int32_t tile_cost) {
+  return tiles == 0 ? 0 : K7_ITEM_COST + tiles * tile_cost;
+}
+__device__ __forceinline__ int32_t k7_cut(int32_t cost, int32_t tile_cost) {
+  return max(cost - K7_ITEM_COST + tile_cost / 2, 0) / tile_cost;
+}
 
 __device__ __forceinline__ int32_t k7_scan_add(int32_t v, int lane) {
 #pragma unroll
@@ -124,8 +145,10 @@ __device__ __forceinline__ void k7_build_plan(const K7Params& p, const K7Plan& p
       const int i = base + lane;
       int32_t b = 0, t = 0;
       if (i < p.n_groups) {
-        b = ((pl.group[i + 1] - pl.group[i]) * p.ratio + K7_ROWS - 1) / K7_ROWS;
-        t = b * p.kv_heads * k7_tiles(k7_length(p, p.prefix_lens[i], p.prefix_blocks));
+        const int32_t rows = (pl.group[i + 1] - pl.group[i]) * p.ratio;
+        b = (rows + K7_ROWS - 1) / K7_ROWS;
+        t = b * p.kv_heads * k7_item_cost(k7_tiles(k7_length(p, p.prefix_lens[i], p.prefix_blocks)),
+                                          k7_tile_cost(rows));
       }
       const int32_t bs = k7_scan_add(b, lane), ts = k7_scan_add(t, lane);
       if (i < p.n_groups) {
@@ -144,7 +167,9 @@ __device__ __forceinline__ void k7_build_plan(const K7Params& p, const K7Plan& p
     for (int base = 0; base < p.n_seq; base += 32) {
       const int i = base + lane;
       int32_t t = 0;
-      if (i < p.n_seq) t = p.kv_heads * k7_tiles(k7_length(p, p.lengths[i], p.seq_blocks));
+      if (i < p.n_seq)
+        t = p.kv_heads * k7_item_cost(k7_tiles(k7_length(p, p.lengths[i], p.seq_blocks)),
+                                      k7_tile_cost(p.ratio));
       const int32_t ts = k7_scan_add(t, lane);
       if (i < p.n_seq) pl.suffix[i] = tiles + ts - t;
       tiles += __shfl_sync(0xffffffffu, ts, 31);
@@ -153,14 +178,14 @@ __device__ __forceinline__ void k7_build_plan(const K7Params& p, const K7Plan& p
   }
 }
 
-// The CTAs that take part (each has a tile, so that an item's pieces lie in neighbouring ones),
-// the first tile of one of them, and the one that holds a tile.
-__device__ __forceinline__ int32_t k7_working(int32_t tiles, int32_t ctas) { return min(tiles, ctas); }
-__device__ __forceinline__ int32_t k7_first_tile(int32_t tiles, int32_t ctas, int32_t cta) {
-  return static_cast<int32_t>(static_cast<int64_t>(cta) * tiles / ctas);
+// The CTAs that take part (each has some cost, so that an item's pieces lie in neighbouring
+// ones), where the run of one begins, and the one that holds a place.
+__device__ __forceinline__ int32_t k7_working(int32_t cost, int32_t ctas) { return min(cost, ctas); }
+__device__ __forceinline__ int32_t k7_begin(int32_t cost, int32_t ctas, int32_t cta) {
+  return static_cast<int32_t>(static_cast<int64_t>(cta) * cost / ctas);
 }
-__device__ __forceinline__ int32_t k7_cta_of(int32_t tiles, int32_t ctas, int32_t tile) {
-  return static_cast<int32_t>(((static_cast<int64_t>(tile) + 1) * ctas + tiles - 1) / tiles - 1);
+__device__ __forceinline__ int32_t k7_cta_of(int32_t cost, int32_t ctas, int32_t place) {
+  return static_cast<int32_t>(((static_cast<int64_t>(place) + 1) * ctas + cost - 1) / cost - 1);
 }
 
 // A piece: tiles [tile, tile + n) of an item.
@@ -168,6 +193,8 @@ struct K7Piece {
   const int32_t* table;
   int32_t len;        // keys of the item
   int32_t tile, n;
+  int32_t tile_cost;
+  int32_t end;        // place where the item ends
   int32_t kv_head;
   int32_t seq0;       // first sequence of the rows
   int32_t row0;       // first row (row = (sequence - seq0) * ratio + head within the KV head)
@@ -186,40 +213,75 @@ __device__ __forceinline__ int k7_find(const int32_t* cum, int n, int32_t x) {
   return lo;
 }
 
-// The piece that begins at tile `at` (of all tiles) and ends at the item's end or at `end`.
-__device__ __forceinline__ K7Piece k7_piece(const K7Params& p, const K7Plan& pl, int32_t at, int32_t end) {
+// Tiles of the item that ends at x.end between the places `at` and `last`.
+__device__ __forceinline__ void k7_cut_piece(K7Piece& x, int32_t at, int32_t last) {
+  const int32_t begin = x.end - k7_item_cost(k7_tiles(x.len), x.tile_cost);
+  x.tile = k7_cut(at - begin, x.tile_cost);
+  x.n = k7_cut(min(last, x.end) - begin, x.tile_cost) - x.tile;
+}
+
+// The part of the item at the place `at` that lies before `last`.
+__device__ __forceinline__ K7Piece k7_piece(const K7Params& p, const K7Plan& pl, int32_t at, int32_t last) {
   K7Piece x;
   const int32_t in_prefix = pl.prefix[p.n_groups];
   x.prefix = at < in_prefix;
   if (x.prefix) {
     const int g = k7_find(pl.prefix, p.n_groups, at);
+    x.seq0 = pl.group[g];
+    const int32_t rows = (pl.group[g + 1] - x.seq0) * p.ratio;
     x.len = k7_length(p, p.prefix_lens[g], p.prefix_blocks);
-    const int32_t tiles = k7_tiles(x.len), rem = at - pl.prefix[g];
-    const int32_t i = rem / tiles;  // (row block, KV head)
-    x.tile = rem - i * tiles;
-    x.n = min(tiles - x.tile, end - at);
+    x.tile_cost = k7_tile_cost(rows);
+    const int32_t cost = k7_item_cost(k7_tiles(x.len), x.tile_cost);
+    const int32_t i = (at - pl.prefix[g]) / cost;  // (row block, KV head)
+    x.end = pl.prefix[g] + (i + 1) * cost;
     const int32_t mb = i / p.kv_heads;
     x.kv_head = i - mb * p.kv_heads;
-    x.seq0 = pl.group[g];
     x.row0 = mb * K7_ROWS;
-    x.rows = min(K7_ROWS, (pl.group[g + 1] - x.seq0) * p.ratio - x.row0);
+    x.rows = min(K7_ROWS, rows - x.row0);
     x.item = (pl.block[g] + mb) * p.kv_heads + x.kv_head;
     x.table = p.prefix_tables + static_cast<int64_t>(g) * p.prefix_blocks;
   } else {
     const int b = k7_find(pl.suffix, p.n_seq, at - in_prefix);
-    x.len = k7_length(p, p.lengths[b], p.seq_blocks);
-    const int32_t tiles = k7_tiles(x.len), rem = at - in_prefix - pl.suffix[b];
-    x.kv_head = rem / tiles;
-    x.tile = rem - x.kv_head * tiles;
-    x.n = min(tiles - x.tile, end - at);
     x.seq0 = b;
+    x.len = k7_length(p, p.lengths[b], p.seq_blocks);
+    x.tile_cost = k7_tile_cost(p.ratio);
+    const int32_t cost = k7_item_cost(k7_tiles(x.len), x.tile_cost), begin = in_prefix + pl.suffix[b];
+    x.kv_head = (at - begin) / cost;
+    x.end = begin + (x.kv_head + 1) * cost;
     x.row0 = 0;
     x.rows = p.ratio;
     x.item = b * p.kv_heads + x.kv_head;
     x.table = p.tables + static_cast<int64_t>(b) * p.seq_blocks;
   }
+  k7_cut_piece(x, at, last);
   return x;
 }
+
+// Next piece with a tile of the run that goes on at `at` (x is the piece before, if `have`); moves
+// `at` behind it.  As a rule it is the next KV head of the same rows and keys, else it is looked up.
+__device__ __forceinline__ bool k7_next(const K7Params& p, const K7Plan& pl, K7Piece& x, bool have,
+                                        int32_t& at, int32_t last) {
+  while (at < last) {
+    if (have && at == x.end && x.kv_head + 1 < p.kv_heads) {
+      x.kv_head += 1;
+      x.item += 1;
+      x.end += k7_item_cost(k7_tiles(x.len), x.tile_cost);
+      k7_cut_piece(x, at, last);
+    } else {
+      x = k7_piece(p, pl, at, last);
+      have = true;
+    }
+    at = min(last, x.end);
+    if (x.n > 0) return true;
+  }
+  return false;
+}
+
+// What the softmax warps need of a piece, written by the first copying thread ahead of them; n = 0
+// behind the last one.
+struct K7Card {
+  int32_t len, tile, n, rows, item, prefix;
+};
 
 // ------------------------------------------------------------------ shared memory and products
 // Tiles of 128-byte rows, 128-byte swizzle: 16-byte piece c of row r of a 64-column block sits
@@ -232,8 +294,8 @@ struct K7Smem {
   static constexpr int P_BYTES = K7_ROWS * K7_KEYS * 2;
   static constexpr int STAGE = 2 * KV_BYTES;
   static constexpr int Q = 0;                              // 2 buffers (piece parity)
-  static constexpr int P = Q + 2 * Q_BYTES;                // 2 buffers (tile parity)
-  static constexpr int KV = P + 2 * P_BYTES;
+  static constexpr int P = Q + 2 * Q_BYTES;
+  static constexpr int KV = P + P_BYTES;
   static constexpr int BARS = KV + K7_STAGES * STAGE;
   static constexpr int FULL = BARS;                        // STAGES
   static constexpr int EMPTY = FULL + K7_STAGES * 8;       // STAGES
@@ -242,8 +304,10 @@ struct K7Smem {
   static constexpr int O_FULL = P_FULL + 16;               // 2
   static constexpr int Q_EMPTY = O_FULL + 16;              // 2
   static constexpr int TMEM = Q_EMPTY + 16;
-  static constexpr int WARP_ML = TMEM + 16;                // [4 warps][16 rows] float2
-  static constexpr int PLAN = WARP_ML + 4 * K7_SMALL_ROWS * 8;
+  static constexpr int WARP_ML = TMEM + 16;                // [4 warps][8 rows] float2
+  static constexpr int CARD_FULL = WARP_ML + K7_SOFTMAX_WARPS * 8 * 8;  // K7_CARDS
+  static constexpr int CARDS = CARD_FULL + K7_CARDS * 8;
+  static constexpr int PLAN = CARDS + K7_CARDS * static_cast<int>(sizeof(K7Card));
   static constexpr int plan_bytes(int n_groups, int n_seq) {
     return 4 * (3 * (n_groups + 1) + n_seq + 1);
   }
@@ -334,7 +398,7 @@ __device__ __forceinline__ void k7_mma(float (&c)[4], const uint32_t (&a)[4], ui
 // barriers; here a tile costs a warp 32 small products and is given back at once.
 template <typename T, int D>
 __device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem, uint32_t base,
-                                               const K7Piece& x, uint32_t& t, uint32_t piece, int warp,
+                                               const K7Card& x, uint32_t& t, uint32_t piece, int warp,
                                                int lane, float* out_o, float2* out_ml) {
   using S = K7Smem<D>;
   const int g = lane >> 2;  // this thread's rows: g and g + 8; its columns: 2 (lane & 3) + {0, 1} of eight
@@ -369,17 +433,37 @@ __device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem,
       if (lane == 0) mbar_arrive(base + S::Q_EMPTY + (piece & 1u) * 8);
     }
     const int32_t valid = x.len - (x.tile + j) * K7_KEYS - warp * 16;  // of this warp's 16 keys
+    // All matrix loads first, then the stage is given back: the ring is as good as one stage
+    // longer, and no load's latency stands before a product.
+    const uint32_t kt = base + S::KV + stage * S::STAGE, vt = kt + S::KV_BYTES;
+    uint32_t kf[D / 16][4], vf[D / 16][4];
     if (valid > 0) {
-      const uint32_t kt = base + S::KV + stage * S::STAGE, vt = kt + S::KV_BYTES;
-      float s[2][4] = {};
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
         const int c = 2 * k + k_c;
-        uint32_t b[4];
-        k7_ldmatrix(kt + (c >> 3) * (K7_KEYS * 128) + k_row * 128 + (((c & 7) ^ (k_row & 7)) << 4), b);
-        k7_mma(s[0], qf[k], b[0], b[1], T());
-        k7_mma(s[1], qf[k], b[2], b[3], T());
+        k7_ldmatrix(kt + (c >> 3) * (K7_KEYS * 128) + k_row * 128 + (((c & 7) ^ (k_row & 7)) << 4), kf[k]);
       }
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) {
+        const int c = 2 * k + v_c;
+        k7_ldmatrix_trans(vt + (c >> 3) * (K7_KEYS * 128) + v_row * 128 + (((c & 7) ^ (v_row & 7)) << 4), vf[k]);
+      }
+    }
+    __syncwarp();
+    if (lane == 0) mbar_arrive(base + S::EMPTY + stage * 8);
+    if (valid > 0) {
+      float s[2][4] = {}, s2[2][4] = {};  // two chains of products for each eight keys
+#pragma unroll
+      for (int k = 0; k < D / 16; k += 2) {
+        k7_mma(s[0], qf[k], kf[k][0], kf[k][1], T());
+        k7_mma(s[1], qf[k], kf[k][2], kf[k][3], T());
+        k7_mma(s2[0], qf[k + 1], kf[k + 1][0], kf[k + 1][1], T());
+        k7_mma(s2[1], qf[k + 1], kf[k + 1][2], kf[k + 1][3], T());
+      }
+#pragma unroll
+      for (int n = 0; n < 2; ++n)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
       if (valid < 16) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -387,18 +471,20 @@ __device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem,
           for (int e = 0; e < 4; ++e)
             if (n * 8 + 2 * (lane & 3) + (e & 1) >= valid) s[n][e] = -INFINITY;
       }
+      // The exponents' reference moves only when a score exceeds it by more than 2^8, which one
+      // vote finds out; the row maxima are formed only then.
       float top[2];
       bool grow = false;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1]));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2)) * p.c;
-        grow |= g + 8 * r < x.rows && (top[r] > ref[r] + 8.0f || (ref[r] == -INFINITY && top[r] > ref[r]));
+        top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])) * p.c;
+        grow |= g + 8 * r < x.rows && (top[r] > ref[r] + 8.0f);
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
+          top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
           const float next = fmaxf(ref[r], top[r]);
           const float alpha = next == -INFINITY ? 1.0f : ex2f(ref[r] - next);
           ref[r] = next;
@@ -422,57 +508,55 @@ __device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem,
         }
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
-        const int c = 2 * i + v_c;
-        uint32_t b[4];
-        k7_ldmatrix_trans(vt + (c >> 3) * (K7_KEYS * 128) + v_row * 128 + (((c & 7) ^ (v_row & 7)) << 4), b);
-        k7_mma(o[2 * i], pf, b[0], b[1], T());
-        k7_mma(o[2 * i + 1], pf, b[2], b[3], T());
+        k7_mma(o[2 * i], pf, vf[i][0], vf[i][1], T());
+        k7_mma(o[2 * i + 1], pf, vf[i][2], vf[i][3], T());
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(base + S::EMPTY + stage * 8);
   }
-  // the warps' results meet in the space of P, which is free between pieces: [warp][row][D], pairs
-  // of a row turned by its index so that the eight rows of a store fall on different banks
+  // The warps' results meet in the space of P, which is free between pieces, eight rows at a time:
+  // [warp][row][D], pairs of a row turned by its index so that the rows of a store fall on
+  // different banks.
   float2* const area = reinterpret_cast<float2*>(smem + S::P);
   float2* const ml = reinterpret_cast<float2*>(smem + S::WARP_ML);
 #pragma unroll
   for (int r = 0; r < 2; ++r) {
+    if (8 * r >= x.rows) break;
     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
     sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-    const int row = g + 8 * r;
-    if (row < x.rows) {
+    if (g + 8 * r < x.rows) {
 #pragma unroll
       for (int i = 0; i < D / 8; ++i)
-        area[(warp * K7_SMALL_ROWS + row) * (D / 2) + ((4 * i + (lane & 3)) ^ ((row & 7) << 2))] =
+        area[(warp * 8 + g) * (D / 2) + ((4 * i + (lane & 3)) ^ (g << 2))] =
             make_float2(o[i][2 * r], o[i][2 * r + 1]);
-      if ((lane & 3) == 0) ml[warp * K7_SMALL_ROWS + row] = make_float2(ref[r], sum[r]);
+      if ((lane & 3) == 0) ml[warp * 8 + g] = make_float2(ref[r], sum[r]);
     }
-  }
-  named_bar_sync(1, K7_SOFTMAX_WARPS * 32);
-  for (int i = warp * 32 + lane; i < x.rows * (D / 2); i += K7_SOFTMAX_WARPS * 32) {
-    const int row = i / (D / 2), f = i - row * (D / 2);
-    float2 w[K7_SOFTMAX_WARPS];
-    float top = -INFINITY;
+    named_bar_sync(1, K7_SOFTMAX_WARPS * 32);
+    const int rows = min(8, x.rows - 8 * r);
+    for (int i = warp * 32 + lane; i < rows * (D / 2); i += K7_SOFTMAX_WARPS * 32) {
+      const int row = i / (D / 2), f = i - row * (D / 2);
+      float2 w[K7_SOFTMAX_WARPS];
+      float top = -INFINITY;
 #pragma unroll
-    for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
-      w[k] = ml[k * K7_SMALL_ROWS + row];
-      top = fmaxf(top, w[k].x);
-    }
-    float2 v = make_float2(0.0f, 0.0f);
-    float l = 0.0f;
+      for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
+        w[k] = ml[k * 8 + row];
+        top = fmaxf(top, w[k].x);
+      }
+      float2 v = make_float2(0.0f, 0.0f);
+      float l = 0.0f;
 #pragma unroll
-    for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
-      const float a = w[k].x == -INFINITY ? (w[k].y == 0.0f ? 0.0f : 1.0f) : ex2f(w[k].x - top);
-      const float2 q = area[(k * K7_SMALL_ROWS + row) * (D / 2) + (f ^ ((row & 7) << 2))];
-      v.x = fmaf(a, q.x, v.x);
-      v.y = fmaf(a, q.y, v.y);
-      l = fmaf(a, w[k].y, l);
+      for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
+        // a warp without a finite score has the weight 0, or 1 where it holds a NaN
+        const float a = w[k].x == -INFINITY ? (w[k].y == 0.0f ? 0.0f : 1.0f) : ex2f(w[k].x - top);
+        const float2 q = area[(k * 8 + row) * (D / 2) + (f ^ (row << 2))];
+        v.x = fmaf(a, q.x, v.x);
+        v.y = fmaf(a, q.y, v.y);
+        l = fmaf(a, w[k].y, l);
+      }
+      *reinterpret_cast<float2*>(out_o + (8 * r + row) * D + 2 * f) = v;
+      if (f == 0) out_ml[8 * r + row] = make_float2(top, l);
     }
-    *reinterpret_cast<float2*>(out_o + row * D + 2 * f) = v;
-    if (f == 0) out_ml[row] = make_float2(top, l);
+    named_bar_sync(1, K7_SOFTMAX_WARPS * 32);  // the space may be written again
   }
-  named_bar_sync(1, K7_SOFTMAX_WARPS * 32);  // P may be written again
   return ok;
 }
 
@@ -490,6 +574,8 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
   pl.prefix = pl.block + p.n_groups + 1;
   pl.suffix = pl.prefix + p.n_groups + 1;
 
+  K7Card* const cards = reinterpret_cast<K7Card*>(smem + S::CARDS);
+
   if (threadIdx.x == K7_MMA_WARP * 32) {
     for (int i = 0; i < K7_STAGES; ++i) {
       mbar_init(base + S::FULL + i * 8, K7_COPY_THREADS);
@@ -501,6 +587,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
       mbar_init(base + S::O_FULL + i * 8, 1);
       mbar_init(base + S::Q_EMPTY + i * 8, K7_SOFTMAX_WARPS);
     }
+    for (int i = 0; i < K7_CARDS; ++i) mbar_init(base + S::CARD_FULL + i * 8, 1);
     fence_mbar_init();
   }
   if (warp == K7_MMA_WARP) {
@@ -513,11 +600,11 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + S::TMEM);
-  const int32_t tiles = pl.prefix[p.n_groups] + pl.suffix[p.n_seq];
-  const int32_t working = k7_working(tiles, p.ctas);
+  const int32_t cost = pl.prefix[p.n_groups] + pl.suffix[p.n_seq];
+  const int32_t working = k7_working(cost, p.ctas);
   const bool works = static_cast<int32_t>(blockIdx.x) < working;
-  const int32_t first = works ? k7_first_tile(tiles, working, blockIdx.x) : 0;
-  const int32_t last = works ? k7_first_tile(tiles, working, blockIdx.x + 1) : 0;
+  const int32_t first = works ? k7_begin(cost, working, blockIdx.x) : 0;
+  const int32_t last = works ? k7_begin(cost, working, blockIdx.x + 1) : 0;
   griddep_launch_dependents();
 
   if (warp < K7_SOFTMAX_WARPS) {
@@ -527,28 +614,34 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
     // counts of tiles (the ring), of tiles and pieces on the tensor core, of all pieces
     uint32_t t = 0, u = 0, big_piece = 0, piece = 0;
     bool ok = true;
-    // the sequences' places for the joining kernel, dealt over the CTAs
+    // For the joining kernel, dealt over the CTAs: where a sequence's items lie.
     for (int b = blockIdx.x * K7_SOFTMAX_WARPS * 32 + threadIdx.x; b < p.n_seq;
          b += gridDim.x * K7_SOFTMAX_WARPS * 32) {
-      int4 a = make_int4(0, 0, 0, 0);  // row within the group, row blocks and tiles before it, tiles per item
+      int4 a = make_int4(0, 0, 0, 0);  // its row within the group, the group's first row block and place, tiles
+      int32_t prefix_tile = K7_SMALL_COST;
       if (p.n_groups > 0 && b >= pl.group[0] && b < pl.group[p.n_groups]) {
         const int g = k7_find(pl.group, p.n_groups, b);
         a = make_int4((b - pl.group[g]) * p.ratio, pl.block[g], pl.prefix[g],
                       k7_tiles(k7_length(p, p.prefix_lens[g], p.prefix_blocks)));
+        prefix_tile = k7_tile_cost((pl.group[g + 1] - pl.group[g]) * p.ratio);
         if (p.prefix_lens[g] > static_cast<int64_t>(p.prefix_blocks) * p.block_size)
           k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);
       }
       const int32_t len = k7_length(p, p.lengths[b], p.seq_blocks);
       if (p.lengths[b] > len) k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);
-      reinterpret_cast<int4*>(p.plan + 4)[b] = a;
-      reinterpret_cast<int2*>(p.plan + 4 + 4 * static_cast<int64_t>(p.n_seq))[b] =
-          make_int2(pl.prefix[p.n_groups] + pl.suffix[b], k7_tiles(len));
+      reinterpret_cast<int4*>(p.plan + 4)[2 * b] = a;
+      reinterpret_cast<int4*>(p.plan + 4)[2 * b + 1] =
+          make_int4(pl.prefix[p.n_groups] + pl.suffix[b], k7_tiles(len), prefix_tile, k7_tile_cost(p.ratio));
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.plan[0] = tiles;
+    if (blockIdx.x == 0 && threadIdx.x == 0) p.plan[0] = cost;
 
-    for (int32_t at = first; at < last && ok; ++piece) {
-      const K7Piece x = k7_piece(p, pl, at, last);
-      at += x.n;
+    for (; ok; ++piece) {
+      if (!mbar_wait(base + S::CARD_FULL + (piece % K7_CARDS) * 8, (piece / K7_CARDS) & 1u)) {
+        k7_raise(p.status, TOME_DEV_TIMEOUT);
+        break;
+      }
+      const K7Card x = cards[piece % K7_CARDS];
+      if (x.n == 0) break;
       const int64_t slot = static_cast<int64_t>(x.item) + blockIdx.x;
       const int64_t rows_at = x.prefix ? slot * K7_ROWS : slot * p.ratio;
       float* const out_o = (x.prefix ? p.prefix_o : p.suffix_o) + rows_at * D;
@@ -565,8 +658,6 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
       float ref = -INFINITY, sum = 0.0f;
       for (int32_t j = 0; j < x.n && ok; ++j, ++t, ++u) {
         const uint32_t buf = u & 1u;
-        // S of this tile; the products before it are done too, P V of the tile before last among them, so
-        // that its buffer of P may be written
         if (!mbar_wait(base + S::S_FULL + buf * 8, (u >> 1) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
           ok = false;
@@ -595,17 +686,20 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * p.c;
           // (lanes beyond the rows hold whatever the last piece left)
           const bool grow = row < x.rows && (top > ref + 8.0f || (j == 0 && top > ref));
+          // P V of the tile before is done: P may be written again, and the sums be rescaled
+          if (j > 0) {
+            if (!mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u)) {
+              k7_raise(p.status, TOME_DEV_TIMEOUT);
+              ok = false;
+            }
+            __syncwarp();
+          }
           if (__any_sync(0xffffffffu, grow)) {
             const float next = grow ? top : ref;
             const float alpha = next == -INFINITY ? 1.0f : ex2f(ref - next);
             sum *= alpha;
             ref = next;
             if (j > 0) {
-              if (!mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u)) {
-                k7_raise(p.status, TOME_DEV_TIMEOUT);
-                ok = false;
-              }
-              __syncwarp();
               tc_fence_after_sync();
 #pragma unroll 1
               for (int h = 0; h < D; h += 32) {
@@ -623,7 +717,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           const float off = ref == -INFINITY ? 0.0f : -ref;
           const float2 c2 = make_float2(p.c, p.c), off2 = make_float2(off, off);
           float2 la = make_float2(0.0f, 0.0f), lb = la;
-          const uint32_t prow = base + S::P + buf * S::P_BYTES + row * 128;
+          const uint32_t prow = base + S::P + row * 128;
 #pragma unroll
           for (int h = 0; h < 8; ++h) {  // eight keys: one 16-byte piece of P
             float2 e[4];
@@ -689,7 +783,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           return;
         }
         tc_fence_after_sync();
-        const uint64_t a = k7_desc_k(base + S::P + buf * S::P_BYTES);
+        const uint64_t a = k7_desc_k(base + S::P);
         const uint64_t b = k7_desc_mn(base + S::KV + pending_stage * S::STAGE + S::KV_BYTES, K7_KEYS * 128);
 #pragma unroll
         for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 32 bytes of a P row, 16 rows of V
@@ -700,9 +794,9 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
         umma_commit(base + S::EMPTY + pending_stage * 8);
         umma_commit(base + S::O_FULL + buf * 8);
       };
-      for (int32_t at = first; at < last && ok; ++piece) {
-        const K7Piece x = k7_piece(p, pl, at, last);
-        at += x.n;
+      K7Piece x;
+      int32_t at = first;
+      for (; ok && k7_next(p, pl, x, piece > 0, at, last); ++piece) {
         if (x.rows <= K7_SMALL_ROWS) {
           if (pending) multiply_pv();
           t += x.n;
@@ -754,28 +848,55 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
     const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
     const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
     const uint32_t area = base + S::KV + (c >> 3) * (K7_KEYS * 128);
-    // Row of the pool (heads and blocks flattened) of key (tile * 64 + my_row + lane), or -1.
-    auto find_row = [&](const K7Piece& x, int32_t tile) -> int32_t {
-      const int32_t key = tile * K7_KEYS + my_row + lane;
-      if (key >= x.len) return -1;
-      const int32_t blk = static_cast<int32_t>((static_cast<uint64_t>(key) * p.div_magic) >> p.div_shift);
-      const int32_t page = __ldg(x.table + blk);
+    auto block_of = [&](int32_t key) {
+      return static_cast<int32_t>(static_cast<uint64_t>(key) * p.div_magic >> p.div_shift);
+    };
+    // 64 entries of the table from block `first` on, two per lane: a tile's pages come from there by
+    // shuffles, and the entries behind them are asked for long before they are needed.
+    struct Pages {
+      int32_t first, a, b;
+    };
+    auto ask = [&](const K7Piece& y, int32_t block) {
+      return block <= block_of(y.len - 1) ? __ldg(y.table + block) : -1;
+    };
+    auto open_pages = [&](const K7Piece& y) {
+      const int32_t f = block_of(min(y.tile * K7_KEYS + my_row, y.len - 1));
+      return Pages{f, ask(y, f + lane), ask(y, f + 32 + lane)};
+    };
+    // The pool's row (blocks and heads flattened) of key (tile * 64 + my_row + lane), or -1.
+    auto pool_row_of = [&](const K7Piece& y, Pages& w, int32_t tile) -> int32_t {
+      const int32_t key0 = tile * K7_KEYS + my_row, key = key0 + lane;
+      if (key0 >= y.len) return -1;
+      const int32_t lo = block_of(key0);
+      if (lo - w.first >= 32) {
+        if (lo - w.first < 64) w = Pages{w.first + 32, w.b, ask(y, w.first + 64 + lane)};
+        else w = Pages{lo, ask(y, lo + lane), ask(y, lo + 32 + lane)};
+      }
+      const int32_t blk = block_of(min(key, y.len - 1)), rel = blk - w.first;  // 0 .. 62
+      const int32_t pa = __shfl_sync(0xffffffffu, w.a, rel & 31), pb = __shfl_sync(0xffffffffu, w.b, rel & 31);
+      const int32_t page = rel < 32 ? pa : pb;
+      if (key >= y.len) return -1;
       if (page < 0 || page >= p.num_blocks) {
         k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);  // reads as zeros, as gather does
         return -1;
       }
-      return (page * p.kv_heads + x.kv_head) * p.block_size + (key - blk * p.block_size);
+      return (page * p.kv_heads + y.kv_head) * p.block_size + (key - blk * p.block_size);
+    };
+    auto show = [&](const K7Piece& y, uint32_t index, bool there) {  // to the softmax warps
+      if (cw == 0 && lane == 0) {
+        cards[index % K7_CARDS] = K7Card{y.len, y.tile, there ? y.n : 0, y.rows, y.item, y.prefix ? 1 : 0};
+        mbar_arrive(base + S::CARD_FULL + (index % K7_CARDS) * 8);
+      }
     };
     uint32_t t = 0, piece = 0;
     bool ok = true;
     int32_t at = first;
-    K7Piece x;
-    int32_t pool_row = -1;
-    if (at < last) {
-      x = k7_piece(p, pl, at, last);
-      pool_row = find_row(x, x.tile);
-    }
-    while (at < last && ok) {
+    K7Piece x = {};
+    Pages pages = {};
+    bool there = k7_next(p, pl, x, false, at, last);
+    show(x, 0, there);
+    if (there) pages = open_pages(x);
+    while (there && ok) {
       if (piece >= 2 && !mbar_wait(base + S::Q_EMPTY + (piece & 1u) * 8, ((piece >> 1) - 1) & 1u)) {
         k7_raise(p.status, TOME_DEV_TIMEOUT);
         ok = false;
@@ -790,16 +911,14 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
                   src, true);
       }
       K7Piece next = x;
-      const int32_t end = at + x.n;
+      Pages next_pages = {};
+      bool next_there = false;
       for (int32_t j = 0; j < x.n; ++j, ++t) {
         const uint32_t stage = t % K7_STAGES;
-        // the next tile's rows are asked for before this one's copies go out
-        int32_t next_row = -1;
-        if (j + 1 < x.n) {
-          next_row = find_row(x, x.tile + j + 1);
-        } else if (end < last) {
-          next = k7_piece(p, pl, end, last);
-          next_row = find_row(next, next.tile);
+        if (j + 1 == x.n) {  // the piece behind is looked up while this one's loads are under way
+          next_there = k7_next(p, pl, next, true, at, last);
+          show(next, piece + 1, next_there);
+          if (next_there) next_pages = open_pages(next);
         }
         if (t >= K7_STAGES && !mbar_wait(base + S::EMPTY + stage * 8, (t / K7_STAGES - 1) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
@@ -807,6 +926,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           break;
         }
         __syncwarp();
+        const int32_t pool_row = pool_row_of(x, pages, x.tile + j);
         const uint32_t dst = area + stage * S::STAGE;
 #pragma unroll
         for (int i = 0; i < STEPS; ++i) {
@@ -818,10 +938,10 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           k7_copy16(to + S::KV_BYTES, v_pool + off, from >= 0);
         }
         k7_copies_arrive(base + S::FULL + stage * 8);
-        pool_row = next_row;
       }
-      at = end;
       x = next;
+      pages = next_pages;
+      there = next_there;
       ++piece;
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -847,23 +967,26 @@ __global__ void __launch_bounds__(128) k7_join_kernel(const K7Params p) {
   if (w >= static_cast<int64_t>(p.n_seq) * p.heads) return;
   const int32_t b = static_cast<int32_t>(w / p.heads), h = static_cast<int32_t>(w - static_cast<int64_t>(b) * p.heads);
   const int32_t kv = h / p.ratio;
-  const int32_t tiles = p.plan[0], working = k7_working(tiles, p.ctas);
-  const int4 a = reinterpret_cast<const int4*>(p.plan + 4)[b];
-  const int2 s = reinterpret_cast<const int2*>(p.plan + 4 + 4 * static_cast<int64_t>(p.n_seq))[b];
+  const int32_t cost = p.plan[0], working = k7_working(cost, p.ctas);
+  const int4 a = reinterpret_cast<const int4*>(p.plan + 4)[2 * b];
+  const int4 s = reinterpret_cast<const int4*>(p.plan + 4)[2 * b + 1];
   const int32_t row = a.x + (h - kv * p.ratio), mb = row / K7_ROWS;
-  int32_t n_prefix = 0, n_suffix = 0;
-  int64_t at_prefix = 0, at_suffix = 0;  // row index of the first piece; pieces are K7_ROWS / ratio rows apart
+  // the CTAs that hold parts of the row's two items, and the row's place in the first one's slot
+  int32_t n_prefix = 0, n_suffix = 0, prefix_cta = 0, suffix_cta = 0, prefix_begin = 0, suffix_begin = 0;
+  int64_t at_prefix = 0, at_suffix = 0;
+  const int32_t prefix_cost = k7_item_cost(a.w, s.z), suffix_cost = k7_item_cost(s.y, s.w);
   if (a.w > 0) {
-    const int32_t i = mb * p.kv_heads + kv, u = a.z + i * a.w;
-    const int32_t c0 = k7_cta_of(tiles, working, u), c1 = k7_cta_of(tiles, working, u + a.w - 1);
-    n_prefix = c1 - c0 + 1;
-    at_prefix = (static_cast<int64_t>(a.y) * p.kv_heads + i + c0) * K7_ROWS + (row - mb * K7_ROWS);
+    const int32_t i = mb * p.kv_heads + kv;
+    prefix_begin = a.z + i * prefix_cost;
+    prefix_cta = k7_cta_of(cost, working, prefix_begin);
+    n_prefix = k7_cta_of(cost, working, prefix_begin + prefix_cost - 1) - prefix_cta + 1;
+    at_prefix = (static_cast<int64_t>(a.y) * p.kv_heads + i + prefix_cta) * K7_ROWS + (row - mb * K7_ROWS);
   }
   if (s.y > 0) {
-    const int32_t u = s.x + kv * s.y;
-    const int32_t c0 = k7_cta_of(tiles, working, u), c1 = k7_cta_of(tiles, working, u + s.y - 1);
-    n_suffix = c1 - c0 + 1;
-    at_suffix = (static_cast<int64_t>(b) * p.kv_heads + kv + c0) * p.ratio + (h - kv * p.ratio);
+    suffix_begin = s.x + kv * suffix_cost;
+    suffix_cta = k7_cta_of(cost, working, suffix_begin);
+    n_suffix = k7_cta_of(cost, working, suffix_begin + suffix_cost - 1) - suffix_cta + 1;
+    at_suffix = (static_cast<int64_t>(b) * p.kv_heads + kv + suffix_cta) * p.ratio + (h - kv * p.ratio);
   }
   const int32_t n = n_prefix + n_suffix;
   float top = -INFINITY, total = 0.0f, acc[E];
@@ -872,8 +995,18 @@ __global__ void __launch_bounds__(128) k7_join_kernel(const K7Params p) {
   for (int32_t base = 0; base < n; base += 32) {
     const int32_t i = base + lane;
     float2 ml = make_float2(-INFINITY, 0.0f);
-    if (i < n_prefix) ml = p.prefix_ml[at_prefix + static_cast<int64_t>(i) * K7_ROWS];
-    else if (i < n) ml = p.suffix_ml[at_suffix + static_cast<int64_t>(i - n_prefix) * p.ratio];
+    bool there = false;  // a CTA's run may hold less than a tile of the item
+    if (i < n) {
+      const bool pre = i < n_prefix;
+      const int32_t cta = pre ? prefix_cta + i : suffix_cta + i - n_prefix;
+      const int32_t begin = pre ? prefix_begin : suffix_begin, end = begin + (pre ? prefix_cost : suffix_cost);
+      const int32_t from = max(k7_begin(cost, working, cta), begin), to = min(k7_begin(cost, working, cta + 1), end);
+      const int32_t w1 = pre ? s.z : s.w;
+      there = k7_cut(to - begin, w1) > k7_cut(from - begin, w1);
+      if (there)
+        ml = pre ? p.prefix_ml[at_prefix + static_cast<int64_t>(i) * K7_ROWS]
+                 : p.suffix_ml[at_suffix + static_cast<int64_t>(i - n_prefix) * p.ratio];
+    }
     if (ml.y == 0.0f) ml.x = -INFINITY;  // a piece that saw nothing but -inf
     float m = ml.x;
 #pragma unroll
@@ -888,10 +1021,12 @@ __global__ void __launch_bounds__(128) k7_join_kernel(const K7Params p) {
     total = fmaf(total, keep, l);
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= keep;
+    const uint32_t which = __ballot_sync(0xffffffffu, there);
     const int32_t here = min(32, n - base);
 #pragma unroll 4
     for (int32_t k = 0; k < here; ++k) {
       const float f = __shfl_sync(0xffffffffu, wgt, k);
+      if (!(which >> k & 1u)) continue;
       const int32_t q = base + k;
       const float* src = q < n_prefix
                              ? p.prefix_o + (at_prefix + static_cast<int64_t>(q) * K7_ROWS) * D
@@ -938,7 +1073,7 @@ static K7Layout k7_layout(int64_t n_seq, int64_t n_groups, int64_t heads, int64_
   const int64_t suffix_slots = n_seq * kv_heads + K7_MAX_CTAS;
   K7Layout l;
   l.plan = 0;
-  l.prefix_o = k7_up(static_cast<size_t>(16 + 24 * n_seq));
+  l.prefix_o = k7_up(static_cast<size_t>(16 + 32 * n_seq));
   l.prefix_ml = l.prefix_o + k7_up(static_cast<size_t>(prefix_slots * K7_ROWS * dim * 4));
   l.suffix_o = l.prefix_ml + k7_up(static_cast<size_t>(prefix_slots * K7_ROWS * 8));
   l.suffix_ml = l.suffix_o + k7_up(static_cast<size_t>(suffix_slots * ratio * dim * 4));
@@ -1025,14 +1160,14 @@ extern "C" int32_t tome_shared_prefix_attention(
   const K7Layout l = k7_layout(n_seq, n_groups, heads, kv_heads, head_dim);
   if (workspace == nullptr || workspace_bytes < l.total)
     return fail(TOME_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, l.total);
-  // tiles in all are counted in 32 bits
+  // the cost of all items is counted in 32 bits
   const int64_t ratio = heads / kv_heads;
-  const int64_t key_tiles = (static_cast<int64_t>(prefix_blocks) * block_size + K7_KEYS - 1) / K7_KEYS;
-  const int64_t seq_tiles = (static_cast<int64_t>(max_blocks) * block_size + K7_KEYS - 1) / K7_KEYS;
+  const int64_t prefix_keys = static_cast<int64_t>(prefix_blocks) * block_size;
+  const int64_t seq_keys = static_cast<int64_t>(max_blocks) * block_size;
   const int64_t row_blocks = n_groups == 0 ? 0 : n_groups + n_seq * ratio / K7_ROWS;
-  if (static_cast<int64_t>(prefix_blocks) * block_size > 0x3fffffff ||
-      static_cast<int64_t>(max_blocks) * block_size > 0x3fffffff ||
-      row_blocks * kv_heads * key_tiles + n_seq * kv_heads * seq_tiles > 0x3fffffff)
+  auto most = [&](int64_t keys) { return K7_ITEM_COST + K7_BIG_COST * ((keys + K7_KEYS - 1) / K7_KEYS); };
+  if (prefix_keys > 0x3fffffff || seq_keys > 0x3fffffff ||
+      row_blocks * kv_heads * most(prefix_keys) + n_seq * kv_heads * most(seq_keys) > 0x3fffffff)
     return fail(TOME_ERR_TOO_LARGE, "the tables name too many keys for one call");
   if (static_cast<int64_t>(num_blocks) * kv_heads > 0x7fffffff / block_size)
     return fail(TOME_ERR_TOO_LARGE, "the pool has more than 2^31 - 1 rows");
