@@ -8,20 +8,16 @@
 //   o = softmax(scale q [K_prefix; K_suffix]^T) [V_prefix; V_suffix].
 //
 // Work.  An item is (KV head, up to 128 query rows that read the same keys): the rows of a
-// group against its prefix, or of one sequence against its suffix.  Items are cut into tiles of
-// 64 keys, weighed by what they cost (an item K7_ITEM_COST, a tile K7_SMALL_COST or K7_BIG_COST, see
-// there) and laid end to end; every CTA takes an equal run of the whole, whatever the lengths: the
-// split follows from the lengths on the device alone.  A CTA's part of an item is a
-// piece; it leaves (sum of p v, row maximum, row sum) in the workspace, and a second kernel
-// joins the pieces of a row.  A row's pieces lie at (item index + CTA index), which no two pieces
-// share since at least one of the two grows from piece to piece.
-//
-// Pipeline of a CTA (one per SM): two warps copy keys and values (16-byte asynchronous copies:
-// pages of any size, rows past the end filled with zeros) into a ring of four stages, one
-// thread issues the tensor-core products S = Q K^T (128 x 64 x D) and O = P V (128 x D x 64),
-// four warps own a row per thread: running maximum and sum, P rounded to the type of V
-// into shared memory; O adds up in tensor memory.  S is double-buffered, so the products
-// of one tile, the softmax of the next and the loads of the ones behind it overlap.
+// group against its prefix, or of one sequence against its suffix.  Items of more than 16 rows are
+// "big": they go through the 5th-generation tensor core, tiles of 64 keys, a CTA at a time.  Items
+// of up to 16 rows are "small": a warp alone takes one, tiles of 16 keys, through warp-level
+// products (on the tensor-core path two to eight rows would cost what 128 do).  The tiles of each
+// kind are laid end to end, and every CTA takes an equal run of the big ones, then each of its
+// twelve warps an equal run of the small ones, whatever the lengths: the split follows from the
+// lengths on the device alone.  A worker's part of an item is a piece; it leaves (sum of p v, row
+// maximum, row sum) in the workspace, and a second kernel joins the pieces of a row.  A piece lies
+// at (item index + worker index), which no two pieces share since at least one of the two grows
+// from piece to piece.
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
 #include <float.h>
@@ -34,24 +30,30 @@
 
 namespace tome {
 
-constexpr int K7_ROWS = 128;   // query rows of an item (TMEM lanes)
-constexpr int K7_KEYS = 64;    // keys of a tile
-constexpr int K7_STAGES = 4;
-constexpr int K7_SOFTMAX_WARPS = 4;
-constexpr int K7_MMA_WARP = 4;
-constexpr int K7_COPY_THREADS = 64;  // a warp fetches half of a tile's keys and values
-constexpr int K7_THREADS = (K7_SOFTMAX_WARPS + 1) * 32 + K7_COPY_THREADS;
-constexpr int K7_SMALL_ROWS = 16;  // pieces of up to this many rows take the warp-level products
-// Costs, in thirds of a tile of few rows: a tile of up to 16 rows, one of more, and what a piece
-// costs besides its tiles (the ring runs dry while the queries come, the warps' results meet).
-constexpr int K7_SMALL_COST = 3;
-constexpr int K7_BIG_COST = 4;
-constexpr int K7_ITEM_COST = 4;
+constexpr int K7_ROWS = 128;         // query rows of a big item at most (TMEM lanes)
+constexpr int K7_SMALL_ROWS = 16;    // of a small one
+constexpr int K7_KEYS = 64;          // keys of a big tile
+constexpr int K7_SMALL_KEYS = 16;    // of a small one
+constexpr int K7_STAGES = 4;         // ring of big tiles
+constexpr int K7_SMALL_STAGES = 2;   // each warp's ring of small tiles
+constexpr int K7_TEAM_WARPS = 4;     // a team takes every other big tile
+constexpr int K7_SOFTMAX_WARPS = 2 * K7_TEAM_WARPS;
+constexpr int K7_QK_WARP = K7_SOFTMAX_WARPS;
+constexpr int K7_COPY_THREADS = 64;  // a warp fetches half of a big tile's keys and values
+constexpr int K7_PV_WARP = K7_QK_WARP + 1 + K7_COPY_THREADS / 32;
+constexpr int K7_WARPS = K7_PV_WARP + 1;         // all of them take small items
+constexpr int K7_THREADS = K7_WARPS * 32;
+// Cost of a small item besides its tiles, in tiles: the warp's ring runs dry where the queries come.
+constexpr int K7_SMALL_ITEM_COST = 2;
 // Cards of pieces in flight.  One is written over four pieces later; the copying warps are at most
 // two pieces ahead of a Q buffer's release, and that comes after the softmax warps took the card.
 constexpr int K7_CARDS = 4;
 constexpr int K7_MAX_SEQ = 2048;
 constexpr int K7_MAX_GROUPS = 512;
+// The split takes at most this many CTAs (one per SM); the workspace does not depend on the
+// device that it is asked for on.
+constexpr int K7_MAX_CTAS = 160;
+constexpr int K7_MAX_WORKERS = K7_MAX_CTAS * K7_WARPS;
 
 struct K7Params {
   const void* q;              // [n_seq, heads, D], sequence stride q_stride
@@ -68,16 +70,20 @@ struct K7Params {
   int32_t div_shift;
   float c;                    // scale * log2(e)
   int32_t ctas;               // CTAs of the main kernel
-  // workspace
-  int32_t* plan;              // [0]: the cost of all items; then two int4 [n_seq], see the kernel
-  float* prefix_o;            // [prefix slots, 128, D]
-  float2* prefix_ml;          // [prefix slots, 128] (maximum * c, sum)
-  float* suffix_o;            // [suffix slots, ratio, D]
-  float2* suffix_ml;          // [suffix slots, ratio]
+  double inv_ctas;            // 1 / ctas
+  // workspace: the pieces' rows, those of big prefix items (128 per piece), of small ones (16) from
+  // row small_rows on, of suffix items (ratio) from row suffix_rows on
+  int4* plan;                 // [n_seq, heads] where a row's pieces are, see K7Where
+  float* part_o;              // [rows, D]
+  float2* part_ml;            // [rows] (maximum * c, sum)
+  int64_t small_rows, suffix_rows;
   void* out;                  // [n_seq, heads, D]
   float* out_lse;             // [n_seq, heads] or null
   int32_t* status;
 };
+
+// A row's record: x, y first row and number of its prefix pieces, z, w of its suffix pieces.  The
+// number of prefix pieces is negative where they are 16 rows apart.
 
 __device__ __forceinline__ void k7_raise(int32_t* status, int32_t bit) {
   if (status != nullptr) atomicOr(status, bit);
@@ -89,27 +95,28 @@ __device__ __forceinline__ int32_t k7_length(const K7Params& p, int32_t len, int
   return static_cast<int32_t>(max(int64_t{0}, min(static_cast<int64_t>(len), most)));
 }
 
+// ------------------------------------------------------------------ the split
+__host__ __device__ constexpr int k7_keys(bool big) { return big ? K7_KEYS : K7_SMALL_KEYS; }
+// Cost of an item besides its tiles.
+__host__ __device__ constexpr int k7_extra(bool big) { return big ? 0 : K7_SMALL_ITEM_COST; }
+
+__device__ __forceinline__ bool k7_is_big(int32_t rows) { return rows > K7_SMALL_ROWS; }
+__device__ __forceinline__ int32_t k7_tiles(int32_t len, bool big) {
+  return (len + k7_keys(big) - 1) / k7_keys(big);
+}
+__device__ __forceinline__ int32_t k7_item_cost(int32_t len, bool big) {
+  return len == 0 ? 0 : k7_extra(big) + k7_tiles(len, big);
+}
+// Tiles that lie before the offset `cost` of an item.
+__device__ __forceinline__ int32_t k7_cut(int32_t cost, bool big) { return max(cost - k7_extra(big), 0); }
+
 // What every CTA works out of the lengths, in shared memory.
 struct K7Plan {
-  int32_t* group;   // [n_groups + 1] first sequence of each group (clamped, not decreasing)
-  int32_t* block;   // [n_groups + 1] row blocks (of 128 rows) before each group
-  int32_t* prefix;  // [n_groups + 1] cost of the prefix items before each group
-  int32_t* suffix;  // [n_seq + 1] cost of the suffix items before each sequence
+  int32_t* group;     // [n_groups + 1] first sequence of each group (clamped, not decreasing)
+  int32_t* block;     // [n_groups + 1] row blocks (of 128 rows) of the big groups before each group
+  int32_t* prefix[2]; // [n_groups + 1] cost of the small [0] and big [1] prefix items before each group
+  int32_t* suffix;    // [n_seq + 1] cost of the suffix items before each sequence
 };
-
-__device__ __forceinline__ int32_t k7_tiles(int32_t len) { return (len + K7_KEYS - 1) / K7_KEYS; }
-
-// Cost of a tile of an item whose rows number `rows`, and of an item; tiles that lie before the
-// offset `cost` of an item.
-__device__ __forceinline__ int32_t k7_tile_cost(int32_t rows) {
-  return rows <= K7_SMALL_ROWS ? K7_SMALL_COST : K7_BIG_COST;
-}
-__device__ __forceinline__ int32_t k7_item_cost(int32_t tiles, int32_t tile_cost) {
-  return tiles == 0 ? 0 : K7_ITEM_COST + tiles * tile_cost;
-}
-__device__ __forceinline__ int32_t k7_cut(int32_t cost, int32_t tile_cost) {
-  return max(cost - K7_ITEM_COST + tile_cost / 2, 0) / tile_cost;
-}
 
 __device__ __forceinline__ int32_t k7_scan_add(int32_t v, int lane) {
 #pragma unroll
@@ -128,64 +135,125 @@ __device__ __forceinline__ int32_t k7_scan_max(int32_t v, int lane) {
   return v;
 }
 
+// Four values per lane from an array of n, 128 from `base` on; 0 past the end.  (All four loads are
+// under way before the first scan waits for one.)
+struct K7Four {
+  int32_t v[4];
+};
+__device__ __forceinline__ K7Four k7_four(const int32_t* src, int n, int base, int lane) {
+  K7Four f;
+#pragma unroll
+  for (int k = 0; k < 4; ++k) f.v[k] = base + 32 * k + lane < n ? __ldg(src + base + 32 * k + lane) : 0;
+  return f;
+}
+
 // Warp 0: the groups; warp 1: the sequences.
 __device__ __forceinline__ void k7_build_plan(const K7Params& p, const K7Plan& pl, int warp, int lane) {
   if (warp == 0) {
+    K7Four len = k7_four(p.prefix_lens, p.n_groups, 0, lane);
     int32_t top = 0;
-    for (int base = 0; base <= p.n_groups; base += 32) {
-      const int i = base + lane;
-      int32_t v = (i <= p.n_groups && p.n_groups > 0) ? p.group_starts[i] : 0;
-      v = max(top, k7_scan_max(min(max(v, 0), p.n_seq), lane));
-      if (i <= p.n_groups) pl.group[i] = v;
-      top = __shfl_sync(0xffffffffu, v, 31);
+    for (int base = 0; base <= p.n_groups; base += 128) {
+      const K7Four f = k7_four(p.group_starts, p.n_groups > 0 ? p.n_groups + 1 : 0, base, lane);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = base + 32 * k + lane;
+        const int32_t v = max(top, k7_scan_max(min(max(f.v[k], 0), p.n_seq), lane));
+        if (i <= p.n_groups) pl.group[i] = v;
+        top = __shfl_sync(0xffffffffu, v, 31);
+      }
     }
     __syncwarp();
-    int32_t blocks = 0, tiles = 0;
-    for (int base = 0; base < p.n_groups; base += 32) {
-      const int i = base + lane;
-      int32_t b = 0, t = 0;
-      if (i < p.n_groups) {
-        const int32_t rows = (pl.group[i + 1] - pl.group[i]) * p.ratio;
-        b = (rows + K7_ROWS - 1) / K7_ROWS;
-        t = b * p.kv_heads * k7_item_cost(k7_tiles(k7_length(p, p.prefix_lens[i], p.prefix_blocks)),
-                                          k7_tile_cost(rows));
+    int32_t blocks = 0, cost[2] = {0, 0};
+    for (int base = 0; base < p.n_groups; base += 128) {
+      if (base > 0) len = k7_four(p.prefix_lens, p.n_groups, base, lane);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = base + 32 * k + lane;
+        if (base + 32 * k >= p.n_groups) break;
+        int32_t b = 0, c[2] = {0, 0};
+        if (i < p.n_groups) {
+          const int32_t rows = (pl.group[i + 1] - pl.group[i]) * p.ratio, n = k7_length(p, len.v[k], p.prefix_blocks);
+          if (k7_is_big(rows)) {
+            b = (rows + K7_ROWS - 1) / K7_ROWS;
+            c[1] = b * p.kv_heads * k7_item_cost(n, true);
+          } else if (rows > 0) {
+            c[0] = p.kv_heads * k7_item_cost(n, false);
+          }
+        }
+        const int32_t bs = k7_scan_add(b, lane);
+        if (i < p.n_groups) pl.block[i] = blocks + bs - b;
+        blocks += __shfl_sync(0xffffffffu, bs, 31);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          const int32_t cs = k7_scan_add(c[s], lane);
+          if (i < p.n_groups) pl.prefix[s][i] = cost[s] + cs - c[s];
+          cost[s] += __shfl_sync(0xffffffffu, cs, 31);
+        }
       }
-      const int32_t bs = k7_scan_add(b, lane), ts = k7_scan_add(t, lane);
-      if (i < p.n_groups) {
-        pl.block[i] = blocks + bs - b;
-        pl.prefix[i] = tiles + ts - t;
-      }
-      blocks += __shfl_sync(0xffffffffu, bs, 31);
-      tiles += __shfl_sync(0xffffffffu, ts, 31);
     }
     if (lane == 0) {
       pl.block[p.n_groups] = blocks;
-      pl.prefix[p.n_groups] = tiles;
+      pl.prefix[0][p.n_groups] = cost[0];
+      pl.prefix[1][p.n_groups] = cost[1];
     }
   } else if (warp == 1) {
-    int32_t tiles = 0;
-    for (int base = 0; base < p.n_seq; base += 32) {
-      const int i = base + lane;
-      int32_t t = 0;
-      if (i < p.n_seq)
-        t = p.kv_heads * k7_item_cost(k7_tiles(k7_length(p, p.lengths[i], p.seq_blocks)),
-                                      k7_tile_cost(p.ratio));
-      const int32_t ts = k7_scan_add(t, lane);
-      if (i < p.n_seq) pl.suffix[i] = tiles + ts - t;
-      tiles += __shfl_sync(0xffffffffu, ts, 31);
+    const bool big = k7_is_big(p.ratio);
+    int32_t cost = 0;
+    for (int base = 0; base < p.n_seq; base += 128) {
+      const K7Four len = k7_four(p.lengths, p.n_seq, base, lane);
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const int i = base + 32 * k + lane;
+        if (base + 32 * k >= p.n_seq) break;
+        const int32_t c = i < p.n_seq ? p.kv_heads * k7_item_cost(k7_length(p, len.v[k], p.seq_blocks), big) : 0;
+        const int32_t cs = k7_scan_add(c, lane);
+        if (i < p.n_seq) pl.suffix[i] = cost + cs - c;
+        cost += __shfl_sync(0xffffffffu, cs, 31);
+      }
     }
-    if (lane == 0) pl.suffix[p.n_seq] = tiles;
+    if (lane == 0) pl.suffix[p.n_seq] = cost;
   }
 }
 
-// The CTAs that take part (each has some cost, so that an item's pieces lie in neighbouring
-// ones), where the run of one begins, and the one that holds a place.
-__device__ __forceinline__ int32_t k7_working(int32_t cost, int32_t ctas) { return min(cost, ctas); }
-__device__ __forceinline__ int32_t k7_begin(int32_t cost, int32_t ctas, int32_t cta) {
-  return static_cast<int32_t>(static_cast<int64_t>(cta) * cost / ctas);
+// Cost of all big or all small items.
+__device__ __forceinline__ int32_t k7_cost(const K7Params& p, const K7Plan& pl, bool big) {
+  return pl.prefix[big][p.n_groups] + (k7_is_big(p.ratio) == big ? pl.suffix[p.n_seq] : 0);
 }
-__device__ __forceinline__ int32_t k7_cta_of(int32_t cost, int32_t ctas, int32_t place) {
-  return static_cast<int32_t>(((static_cast<int64_t>(place) + 1) * ctas + cost - 1) / cost - 1);
+
+// The split of a kind's cost over the workers that take part: where the run of one begins, and the
+// one that holds a place.  Every run is long enough to hold a tile of any item it goes through, but
+// for the item's first and last run.  Quotients of up to 2^41 by products with a reciprocal, put
+// right by one.
+struct K7Split {
+  int32_t cost, workers;
+  double inv_workers;
+  __device__ __forceinline__ K7Split(int32_t all, int32_t most, double inv_most, bool big)
+      : cost(all),
+        workers(all == 0 ? 0 : min(max(all / (k7_extra(big) + 1), 1), most)),
+        inv_workers(workers == most ? inv_most : 1.0 / max(workers, 1)) {}
+  static __device__ __forceinline__ int32_t quotient(int64_t a, int32_t b, double inv) {
+    int64_t q = static_cast<int64_t>(static_cast<double>(a) * inv);
+    const int64_t r = a - q * b;
+    q += (r >= b) - (r < 0);
+    return static_cast<int32_t>(q);
+  }
+  __device__ __forceinline__ int32_t begin(int32_t worker) const {
+    return quotient(static_cast<int64_t>(worker) * cost, workers, inv_workers);
+  }
+  // the last worker that begins at the place or before it
+  __device__ __forceinline__ int32_t holder(int32_t place) const {
+    return quotient((static_cast<int64_t>(place) + 1) * workers - 1, cost, 1.0 / cost);
+  }
+};
+
+// First of the workers that hold tiles of the item of `len` > 0 keys that begins at the place
+// `begin`, and how many do.  (The first and the last run may hold less than a tile of it.)
+__device__ __forceinline__ int2 k7_holders(const K7Split& split, int32_t begin, int32_t len, bool big) {
+  const int32_t cost = k7_item_cost(len, big);
+  int32_t w0 = split.holder(begin), w1 = split.holder(begin + cost - 1);
+  if (k7_cut(min(split.begin(w0 + 1) - begin, cost), big) == 0) ++w0;
+  if (k7_cut(max(split.begin(w1) - begin, 0), big) == k7_tiles(len, big)) --w1;
+  return make_int2(w0, w1 - w0 + 1);
 }
 
 // A piece: tiles [tile, tile + n) of an item.
@@ -193,13 +261,12 @@ struct K7Piece {
   const int32_t* table;
   int32_t len;        // keys of the item
   int32_t tile, n;
-  int32_t tile_cost;
   int32_t end;        // place where the item ends
   int32_t kv_head;
   int32_t seq0;       // first sequence of the rows
   int32_t row0;       // first row (row = (sequence - seq0) * ratio + head within the KV head)
   int32_t rows;
-  int32_t item;       // index among the prefix or suffix items
+  int32_t item;       // index among the big prefix, small prefix or suffix items
   bool prefix;
 };
 
@@ -214,38 +281,38 @@ __device__ __forceinline__ int k7_find(const int32_t* cum, int n, int32_t x) {
 }
 
 // Tiles of the item that ends at x.end between the places `at` and `last`.
-__device__ __forceinline__ void k7_cut_piece(K7Piece& x, int32_t at, int32_t last) {
-  const int32_t begin = x.end - k7_item_cost(k7_tiles(x.len), x.tile_cost);
-  x.tile = k7_cut(at - begin, x.tile_cost);
-  x.n = k7_cut(min(last, x.end) - begin, x.tile_cost) - x.tile;
+__device__ __forceinline__ void k7_cut_piece(K7Piece& x, int32_t at, int32_t last, bool big) {
+  const int32_t begin = x.end - k7_item_cost(x.len, big);
+  x.tile = k7_cut(at - begin, big);
+  x.n = k7_cut(min(last, x.end) - begin, big) - x.tile;
 }
 
 // The part of the item at the place `at` that lies before `last`.
-__device__ __forceinline__ K7Piece k7_piece(const K7Params& p, const K7Plan& pl, int32_t at, int32_t last) {
+template <bool BIG>
+__device__ __noinline__ K7Piece k7_piece(const K7Params& p, const K7Plan& pl, int32_t at, int32_t last) {
   K7Piece x;
-  const int32_t in_prefix = pl.prefix[p.n_groups];
+  const int32_t* cum = pl.prefix[BIG];
+  const int32_t in_prefix = cum[p.n_groups];
   x.prefix = at < in_prefix;
   if (x.prefix) {
-    const int g = k7_find(pl.prefix, p.n_groups, at);
+    const int g = k7_find(cum, p.n_groups, at);
     x.seq0 = pl.group[g];
     const int32_t rows = (pl.group[g + 1] - x.seq0) * p.ratio;
     x.len = k7_length(p, p.prefix_lens[g], p.prefix_blocks);
-    x.tile_cost = k7_tile_cost(rows);
-    const int32_t cost = k7_item_cost(k7_tiles(x.len), x.tile_cost);
-    const int32_t i = (at - pl.prefix[g]) / cost;  // (row block, KV head)
-    x.end = pl.prefix[g] + (i + 1) * cost;
-    const int32_t mb = i / p.kv_heads;
+    const int32_t cost = k7_item_cost(x.len, BIG);
+    const int32_t i = (at - cum[g]) / cost;  // (row block, KV head)
+    x.end = cum[g] + (i + 1) * cost;
+    const int32_t mb = i / p.kv_heads;       // 0 for a small item
     x.kv_head = i - mb * p.kv_heads;
     x.row0 = mb * K7_ROWS;
     x.rows = min(K7_ROWS, rows - x.row0);
-    x.item = (pl.block[g] + mb) * p.kv_heads + x.kv_head;
+    x.item = ((BIG ? pl.block[g] : g) + mb) * p.kv_heads + x.kv_head;
     x.table = p.prefix_tables + static_cast<int64_t>(g) * p.prefix_blocks;
   } else {
     const int b = k7_find(pl.suffix, p.n_seq, at - in_prefix);
     x.seq0 = b;
     x.len = k7_length(p, p.lengths[b], p.seq_blocks);
-    x.tile_cost = k7_tile_cost(p.ratio);
-    const int32_t cost = k7_item_cost(k7_tiles(x.len), x.tile_cost), begin = in_prefix + pl.suffix[b];
+    const int32_t cost = k7_item_cost(x.len, BIG), begin = in_prefix + pl.suffix[b];
     x.kv_head = (at - begin) / cost;
     x.end = begin + (x.kv_head + 1) * cost;
     x.row0 = 0;
@@ -253,22 +320,23 @@ __device__ __forceinline__ K7Piece k7_piece(const K7Params& p, const K7Plan& pl,
     x.item = b * p.kv_heads + x.kv_head;
     x.table = p.tables + static_cast<int64_t>(b) * p.seq_blocks;
   }
-  k7_cut_piece(x, at, last);
+  k7_cut_piece(x, at, last, BIG);
   return x;
 }
 
 // Next piece with a tile of the run that goes on at `at` (x is the piece before, if `have`); moves
 // `at` behind it.  As a rule it is the next KV head of the same rows and keys, else it is looked up.
+template <bool BIG>
 __device__ __forceinline__ bool k7_next(const K7Params& p, const K7Plan& pl, K7Piece& x, bool have,
                                         int32_t& at, int32_t last) {
   while (at < last) {
     if (have && at == x.end && x.kv_head + 1 < p.kv_heads) {
       x.kv_head += 1;
       x.item += 1;
-      x.end += k7_item_cost(k7_tiles(x.len), x.tile_cost);
-      k7_cut_piece(x, at, last);
+      x.end += k7_item_cost(x.len, BIG);
+      k7_cut_piece(x, at, last, BIG);
     } else {
-      x = k7_piece(p, pl, at, last);
+      x = k7_piece<BIG>(p, pl, at, last);
       have = true;
     }
     at = min(last, x.end);
@@ -277,8 +345,58 @@ __device__ __forceinline__ bool k7_next(const K7Params& p, const K7Plan& pl, K7P
   return false;
 }
 
-// What the softmax warps need of a piece, written by the first copying thread ahead of them; n = 0
-// behind the last one.
+// First of the workspace's rows that belong to a piece.
+__device__ __forceinline__ int64_t k7_out_row(const K7Params& p, bool prefix, bool big, int32_t item, int32_t worker) {
+  const int64_t slot = static_cast<int64_t>(item) + worker;
+  if (!prefix) return p.suffix_rows + slot * p.ratio;
+  return big ? slot * K7_ROWS : p.small_rows + slot * K7_SMALL_ROWS;
+}
+
+// Pages of keys.  64 entries of the table from block `first` on, two per lane: a tile's pages come
+// from there by shuffles, and the entries behind them are asked for long before they are needed.
+struct K7Pages {
+  int32_t first, a, b;
+};
+__device__ __forceinline__ int32_t k7_block(const K7Params& p, int32_t key) {
+  return static_cast<int32_t>(static_cast<uint64_t>(key) * p.div_magic >> p.div_shift);
+}
+__device__ __forceinline__ int32_t k7_entry(const K7Params& p, const K7Piece& y, int32_t block) {
+  return block <= k7_block(p, y.len - 1) ? __ldg(y.table + block) : -1;
+}
+__device__ __forceinline__ K7Pages k7_open_pages(const K7Params& p, const K7Piece& y, int32_t key0, int lane) {
+  const int32_t f = k7_block(p, min(key0, y.len - 1));
+  return K7Pages{f, k7_entry(p, y, f + lane), k7_entry(p, y, f + 32 + lane)};
+}
+// Moves the entries on so that `block`, which does not fall from call to call, is among the first 32.
+__device__ __forceinline__ void k7_turn_pages(const K7Params& p, const K7Piece& y, K7Pages& w, int32_t block, int lane) {
+  if (block - w.first < 32) return;
+  if (block - w.first < 64) w = K7Pages{w.first + 32, w.b, k7_entry(p, y, w.first + 64 + lane)};
+  else w = K7Pages{block, k7_entry(p, y, block + lane), k7_entry(p, y, block + 32 + lane)};
+}
+// The page of `block` (the same for the whole warp).
+__device__ __forceinline__ int32_t k7_page(const K7Params& p, const K7Piece& y, K7Pages& w, int32_t block, int lane) {
+  k7_turn_pages(p, y, w, block, lane);
+  return __shfl_sync(0xffffffffu, w.a, block - w.first);
+}
+// The pool's row (blocks and heads flattened) of key (key0 + lane), or -1; key0 does not fall from
+// call to call, and no more than 32 keys from it on are asked for.
+__device__ __forceinline__ int32_t k7_pool_row(const K7Params& p, const K7Piece& y, K7Pages& w, int32_t key0, int lane) {
+  if (key0 >= y.len) return -1;
+  const int32_t key = key0 + lane, lo = k7_block(p, key0);
+  k7_turn_pages(p, y, w, lo, lane);
+  const int32_t blk = k7_block(p, min(key, y.len - 1)), rel = blk - w.first;  // 0 .. 62
+  const int32_t pa = __shfl_sync(0xffffffffu, w.a, rel & 31), pb = __shfl_sync(0xffffffffu, w.b, rel & 31);
+  const int32_t page = rel < 32 ? pa : pb;
+  if (key >= y.len) return -1;
+  if (page < 0 || page >= p.num_blocks) {
+    k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);  // reads as zeros, as gather does
+    return -1;
+  }
+  return (page * p.kv_heads + y.kv_head) * p.block_size + (key - blk * p.block_size);
+}
+
+// What the softmax warps need of a big piece, written by the first copying thread ahead of them;
+// n = 0 behind the last one.
 struct K7Card {
   int32_t len, tile, n, rows, item, prefix;
 };
@@ -288,28 +406,35 @@ struct K7Card {
 // at r * 128 + ((c ^ (r & 7)) << 4).
 template <int D>
 struct K7Smem {
-  static constexpr int TMEM_COLS = D == 64 ? 256 : 512;    // S 2 x 64, O 2 x D, a power of two
+  // tensor memory: S 2 x 64 columns, O 2 x D, P 2 x 32 (two 16-bit values per column)
+  static constexpr int O_COL = 2 * K7_KEYS;
+  static constexpr int P_COL = O_COL + 2 * D;
+  static constexpr int TMEM_COLS = 512;
   static constexpr int Q_BYTES = K7_ROWS * D * 2;
   static constexpr int KV_BYTES = K7_KEYS * D * 2;
-  static constexpr int P_BYTES = K7_ROWS * K7_KEYS * 2;
   static constexpr int STAGE = 2 * KV_BYTES;
   static constexpr int Q = 0;                              // 2 buffers (piece parity)
-  static constexpr int P = Q + 2 * Q_BYTES;
-  static constexpr int KV = P + P_BYTES;
-  static constexpr int BARS = KV + K7_STAGES * STAGE;
+  static constexpr int KV = Q + 2 * Q_BYTES;
+  // small items: each warp's ring of tiles lies in the same space
+  static constexpr int SMALL_KV = K7_SMALL_KEYS * D * 2;
+  static constexpr int SMALL_STAGE = 2 * SMALL_KV;
+  static constexpr int SMALL = K7_WARPS * K7_SMALL_STAGES * SMALL_STAGE;
+  static constexpr int MEET_ML = KV + K7_STAGES * STAGE;   // [2 teams][128] float2
+  static_assert(SMALL <= MEET_ML, "small tiles");
+  static constexpr int BARS = MEET_ML + 2 * K7_ROWS * 8;
   static constexpr int FULL = BARS;                        // STAGES
   static constexpr int EMPTY = FULL + K7_STAGES * 8;       // STAGES
-  static constexpr int S_FULL = EMPTY + K7_STAGES * 8;     // 2
-  static constexpr int P_FULL = S_FULL + 16;               // 2
-  static constexpr int O_FULL = P_FULL + 16;               // 2
+  static constexpr int S_FULL = EMPTY + K7_STAGES * 8;     // 2 (teams), as the next two
+  static constexpr int P_FULL = S_FULL + 16;
+  static constexpr int O_FULL = P_FULL + 16;
   static constexpr int Q_EMPTY = O_FULL + 16;              // 2
-  static constexpr int TMEM = Q_EMPTY + 16;
-  static constexpr int WARP_ML = TMEM + 16;                // [4 warps][8 rows] float2
-  static constexpr int CARD_FULL = WARP_ML + K7_SOFTMAX_WARPS * 8 * 8;  // K7_CARDS
+  static constexpr int MEET = Q_EMPTY + 16;                // the softmax warps among themselves
+  static constexpr int TMEM = MEET + 16;
+  static constexpr int CARD_FULL = TMEM + 16;              // K7_CARDS
   static constexpr int CARDS = CARD_FULL + K7_CARDS * 8;
   static constexpr int PLAN = CARDS + K7_CARDS * static_cast<int>(sizeof(K7Card));
   static constexpr int plan_bytes(int n_groups, int n_seq) {
-    return 4 * (3 * (n_groups + 1) + n_seq + 1);
+    return 4 * (4 * (n_groups + 1) + n_seq + 1);
   }
 };
 
@@ -391,80 +516,157 @@ __device__ __forceinline__ void k7_mma(float (&c)[4], const uint32_t (&a)[4], ui
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
-// A piece of up to 16 rows (a sequence's own tokens, as a rule two to eight rows): each of the
-// four warps takes 16 keys of every tile through warp-level products, with its own running
-// maximum and sum and its sums of p v in registers; they meet at the end of the piece.  The
-// tensor-core path below would compute 128 rows for these few and pass each tile through four
-// barriers; here a tile costs a warp 32 small products and is given back at once.
+// All softmax warps meet: what each wrote before is visible to all behind.  An mbarrier rather than
+// a hardware barrier, so that the wait has a limit too; `met` counts the meetings.
+__device__ __forceinline__ void k7_meet(const K7Params& p, uint32_t bar, uint32_t& met, int lane, bool& ok) {
+  __syncwarp();
+  if (lane == 0) mbar_arrive(bar);
+  if (ok && !mbar_wait(bar, met & 1u)) {
+    k7_raise(p.status, TOME_DEV_TIMEOUT);
+    ok = false;
+  }
+  ++met;
+  __syncwarp();
+}
+
+// ------------------------------------------------------------------ small items
+// A warp's run of small tiles.  It copies its own keys and values, a tile ahead, and keeps running
+// maximum, sum and the sums of p v in registers: nothing is shared with another warp, and twelve of
+// them hide one another's latencies.  What counts is the number of instructions per tile, since a
+// warp issues about one in eight clocks: addresses are formed once, and a tile that lies within a
+// page (pages of a multiple of 16 tokens) is copied from one address on.
 template <typename T, int D>
-__device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem, uint32_t base,
-                                               const K7Card& x, uint32_t& t, uint32_t piece, int warp,
-                                               int lane, float* out_o, float2* out_ml) {
+__device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl, uint32_t ring, int32_t worker,
+                                             int32_t first, int32_t last, int lane) {
   using S = K7Smem<D>;
+  constexpr int PIECES = D / 8;                     // 16-byte pieces of a row
+  constexpr int AT_ONCE = 32 / PIECES;              // rows copied per step
+  constexpr int STEPS = K7_SMALL_KEYS / AT_ONCE;
+  constexpr int BLOCK = K7_SMALL_KEYS * 128;        // bytes of a 64-column block of a tile
+  // the copying side, two tiles ahead of the products
+  K7Piece cp = {};
+  int32_t cp_at = first, cp_j = 0;
+  K7Pages pages = {};
+  bool cp_there = k7_next<false>(p, pl, cp, false, cp_at, last);
+  if (cp_there) pages = k7_open_pages(p, cp, cp.tile * K7_SMALL_KEYS, lane);
+  const int c = lane % PIECES, sub = lane / PIECES;
+  const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
+  const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
+  const bool whole_pages = p.block_size % K7_SMALL_KEYS == 0;
+  // places in a tile of the rows r = i * AT_ONCE + sub, which repeat every eight rows
+  constexpr int TURN = 8 / AT_ONCE;
+  uint32_t spot[TURN];
+#pragma unroll
+  for (int i = 0; i < TURN; ++i) {
+    const int r = i * AT_ONCE + sub;
+    spot[i] = ring + (c >> 3) * BLOCK + r * 128 + (((c & 7) ^ r) << 4);
+  }
+  uint32_t fill_at = 0;  // offset of the ring's stage that is filled next
+  auto fill = [&]() {    // the next tile into the ring (or nothing); always one group of copies
+    if (cp_there) {
+      const int32_t key0 = (cp.tile + cp_j) * K7_SMALL_KEYS;
+      bool done = false;
+      if (whole_pages && key0 + K7_SMALL_KEYS <= cp.len) {
+        const int32_t blk = k7_block(p, key0);
+        const int32_t page = k7_page(p, cp, pages, blk, lane);
+        if (page >= 0 && page < p.num_blocks) {
+          const int64_t off = (static_cast<int64_t>(page * p.kv_heads + cp.kv_head) * p.block_size +
+                               (key0 - blk * p.block_size) + sub) * D;
+          const T* kp = k_pool + off;
+          const T* vp = v_pool + off;
+#pragma unroll
+          for (int i = 0; i < STEPS; ++i) {
+            const uint32_t to = spot[i % TURN] + fill_at + (i / TURN) * 1024;
+            k7_copy16(to, kp + i * AT_ONCE * D, true);
+            k7_copy16(to + S::SMALL_KV, vp + i * AT_ONCE * D, true);
+          }
+          done = true;
+        }
+      }
+      if (!done) {
+        const int32_t row = k7_pool_row(p, cp, pages, key0, lane);
+#pragma unroll 1
+        for (int i = 0; i < STEPS; ++i) {
+          const int r = i * AT_ONCE + sub;
+          const int32_t from = __shfl_sync(0xffffffffu, row, r);
+          const int64_t off = static_cast<int64_t>(max(from, 0)) * D;
+          const uint32_t to = ring + fill_at + (c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          k7_copy16(to, k_pool + off, from >= 0);
+          k7_copy16(to + S::SMALL_KV, v_pool + off, from >= 0);
+        }
+      }
+      fill_at = S::SMALL_STAGE - fill_at;
+      if (++cp_j == cp.n) {
+        cp_there = k7_next<false>(p, pl, cp, true, cp_at, last);
+        cp_j = 0;
+        if (cp_there) pages = k7_open_pages(p, cp, cp.tile * K7_SMALL_KEYS, lane);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+  fill();
+
   const int g = lane >> 2;  // this thread's rows: g and g + 8; its columns: 2 (lane & 3) + {0, 1} of eight
-  bool ok = true;
-  uint32_t qf[D / 16][4];
-  float o[D / 8][4];
+  const int k_row = (lane & 7) + ((lane >> 4) << 3), k_c = (lane >> 3) & 1;  // where the lane points
+  const int v_row = lane & 15, v_c = lane >> 4;                              // the matrix loads to
+  // places in a tile that the lane's matrix loads read: column pairs k, k + 4 lie a block apart
+  uint32_t k_spot[4], v_spot[4];
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i)
+  for (int k = 0; k < 4; ++k) {
+    k_spot[k] = ring + k_row * 128 + (((2 * k + k_c) ^ (k_row & 7)) << 4);
+    v_spot[k] = ring + S::SMALL_KV + v_row * 128 + (((2 * k + v_c) ^ (v_row & 7)) << 4);
+  }
+  K7Piece x = {};
+  int32_t at = first;
+  uint32_t read_at = 0;
+  for (bool have = false; k7_next<false>(p, pl, x, have, at, last); have = true) {
+    // queries, straight into the products' layout
+    uint32_t qf[D / 16][4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) o[i][e] = 0.0f;
-  float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
-  // where this lane points the matrix loads to: row and 16-byte piece of Q, K and V tiles
-  const int q_row = lane & 15, q_c = lane >> 4;
-  const int k_row = warp * 16 + (lane & 7) + ((lane >> 4) << 3), k_c = (lane >> 3) & 1;
-  const int v_row = warp * 16 + (lane & 15), v_c = lane >> 4;
-  for (int32_t j = 0; j < x.n; ++j, ++t) {
-    const uint32_t stage = t % K7_STAGES;
-    if (ok && !mbar_wait(base + S::FULL + stage * 8, (t / K7_STAGES) & 1u)) {
-      k7_raise(p.status, TOME_DEV_TIMEOUT);
-      ok = false;
-    }
-    __syncwarp();
-    if (j == 0) {  // the queries came with the first tile
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int c = 2 * k + q_c;
-        k7_ldmatrix(base + S::Q + (piece & 1u) * S::Q_BYTES + (c >> 3) * (K7_ROWS * 128) + q_row * 128 +
-                        (((c & 7) ^ (q_row & 7)) << 4),
-                    qf[k]);
-      }
-      __syncwarp();
-      if (lane == 0) mbar_arrive(base + S::Q_EMPTY + (piece & 1u) * 8);
-    }
-    const int32_t valid = x.len - (x.tile + j) * K7_KEYS - warp * 16;  // of this warp's 16 keys
-    // All matrix loads first, then the stage is given back: the ring is as good as one stage
-    // longer, and no load's latency stands before a product.
-    const uint32_t kt = base + S::KV + stage * S::STAGE, vt = kt + S::KV_BYTES;
-    uint32_t kf[D / 16][4], vf[D / 16][4];
-    if (valid > 0) {
+    for (int r = 0; r < 2; ++r) {
+      const int32_t row = g + 8 * r, s = row / p.ratio;
+      const uint32_t* src = reinterpret_cast<const uint32_t*>(
+          reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
+          static_cast<int64_t>(x.kv_head * p.ratio + (row - s * p.ratio)) * D) + (lane & 3);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        const int c = 2 * k + k_c;
-        k7_ldmatrix(kt + (c >> 3) * (K7_KEYS * 128) + k_row * 128 + (((c & 7) ^ (k_row & 7)) << 4), kf[k]);
-      }
-#pragma unroll
-      for (int k = 0; k < D / 16; ++k) {
-        const int c = 2 * k + v_c;
-        k7_ldmatrix_trans(vt + (c >> 3) * (K7_KEYS * 128) + v_row * 128 + (((c & 7) ^ (v_row & 7)) << 4), vf[k]);
+        qf[k][r] = row < x.rows ? __ldg(src + 8 * k) : 0u;
+        qf[k][2 + r] = row < x.rows ? __ldg(src + 8 * k + 4) : 0u;
       }
     }
-    __syncwarp();
-    if (lane == 0) mbar_arrive(base + S::EMPTY + stage * 8);
-    if (valid > 0) {
+    float o[D / 8][4];
+#pragma unroll
+    for (int k = 0; k < D / 8; ++k)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[k][e] = 0.0f;
+    float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
+#pragma unroll 1
+    for (int32_t j = 0; j < x.n; ++j) {
+      __syncwarp();  // the tile before, whose place is filled now, is done with
+      fill();
+      asm volatile("cp.async.wait_group 1;" ::: "memory");
+      __syncwarp();  // every lane's copies of this tile have landed
       float s[2][4] = {}, s2[2][4] = {};  // two chains of products for each eight keys
+      uint32_t f[D / 16][4];
+      // all loads of the keys first: no load's latency stands before a product
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) k7_ldmatrix(k_spot[k % 4] + read_at + (k / 4) * BLOCK, f[k]);
 #pragma unroll
       for (int k = 0; k < D / 16; k += 2) {
-        k7_mma(s[0], qf[k], kf[k][0], kf[k][1], T());
-        k7_mma(s[1], qf[k], kf[k][2], kf[k][3], T());
-        k7_mma(s2[0], qf[k + 1], kf[k + 1][0], kf[k + 1][1], T());
-        k7_mma(s2[1], qf[k + 1], kf[k + 1][2], kf[k + 1][3], T());
+        k7_mma(s[0], qf[k], f[k][0], f[k][1], T());
+        k7_mma(s[1], qf[k], f[k][2], f[k][3], T());
+        k7_mma(s2[0], qf[k + 1], f[k + 1][0], f[k + 1][1], T());
+        k7_mma(s2[1], qf[k + 1], f[k + 1][2], f[k + 1][3], T());
       }
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k) k7_ldmatrix_trans(v_spot[k % 4] + read_at + (k / 4) * BLOCK, f[k]);
+      read_at = S::SMALL_STAGE - read_at;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
-      if (valid < 16) {
+      const int32_t valid = x.len - (x.tile + j) * K7_SMALL_KEYS;
+      if (valid < K7_SMALL_KEYS) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -478,7 +680,7 @@ __device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem,
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])) * p.c;
-        grow |= g + 8 * r < x.rows && (top[r] > ref[r] + 8.0f);
+        grow |= top[r] > ref[r] + 8.0f;
       }
       if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
@@ -490,12 +692,13 @@ __device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem,
           ref[r] = next;
           sum[r] *= alpha;
 #pragma unroll
-          for (int i = 0; i < D / 8; ++i) {
-            o[i][2 * r] *= alpha;
-            o[i][2 * r + 1] *= alpha;
+          for (int k = 0; k < D / 8; ++k) {
+            o[k][2 * r] *= alpha;
+            o[k][2 * r + 1] *= alpha;
           }
         }
       }
+      // a row that has seen nothing but -inf takes 0 as its reference: all its p are 0
       const float off[2] = {ref[0] == -INFINITY ? 0.0f : -ref[0], ref[1] == -INFINITY ? 0.0f : -ref[1]};
       uint32_t pf[4];
 #pragma unroll
@@ -507,59 +710,171 @@ __device__ __forceinline__ bool k7_small_piece(const K7Params& p, uint8_t* smem,
           pf[2 * n + r] = k7_pack(a, b, T());
         }
 #pragma unroll
-      for (int i = 0; i < D / 16; ++i) {
-        k7_mma(o[2 * i], pf, vf[i][0], vf[i][1], T());
-        k7_mma(o[2 * i + 1], pf, vf[i][2], vf[i][3], T());
+      for (int k = 0; k < D / 16; ++k) {
+        k7_mma(o[2 * k], pf, f[k][0], f[k][1], T());
+        k7_mma(o[2 * k + 1], pf, f[k][2], f[k][3], T());
+      }
+    }
+    const int64_t out_row = k7_out_row(p, x.prefix, false, x.item, worker);
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
+      sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
+      if (g + 8 * r < x.rows) {
+        float* dst = p.part_o + (out_row + g + 8 * r) * D + 2 * (lane & 3);
+#pragma unroll
+        for (int k = 0; k < D / 8; ++k) *reinterpret_cast<float2*>(dst + 8 * k) = make_float2(o[k][2 * r], o[k][2 * r + 1]);
+        if ((lane & 3) == 0) p.part_ml[out_row + g + 8 * r] = make_float2(ref[r], sum[r]);
       }
     }
   }
-  // The warps' results meet in the space of P, which is free between pieces, eight rows at a time:
-  // [warp][row][D], pairs of a row turned by its index so that the rows of a store fall on
-  // different banks.
-  float2* const area = reinterpret_cast<float2*>(smem + S::P);
-  float2* const ml = reinterpret_cast<float2*>(smem + S::WARP_ML);
-#pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    if (8 * r >= x.rows) break;
-    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
-    sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-    if (g + 8 * r < x.rows) {
-#pragma unroll
-      for (int i = 0; i < D / 8; ++i)
-        area[(warp * 8 + g) * (D / 2) + ((4 * i + (lane & 3)) ^ (g << 2))] =
-            make_float2(o[i][2 * r], o[i][2 * r + 1]);
-      if ((lane & 3) == 0) ml[warp * 8 + g] = make_float2(ref[r], sum[r]);
+  asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// ------------------------------------------------------------------ big items
+// Softmax of a piece: thread = row, the team's tiles in turn.
+template <typename T, int D>
+__device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, uint32_t base, uint32_t tmem,
+                                             const K7Card& x, uint32_t& u, int warp, int lane,
+                                             float* out_o, float2* out_ml, uint32_t& met) {
+  using S = K7Smem<D>;
+  const uint32_t team = warp / K7_TEAM_WARPS;
+  const int row = (warp % K7_TEAM_WARPS) * 32 + lane;
+  const uint32_t lanes = static_cast<uint32_t>((warp % K7_TEAM_WARPS) * 32) << 16;
+  const bool active = (warp % K7_TEAM_WARPS) * 32 < x.rows;  // warps without a row only keep step
+  const uint32_t o_addr = tmem + lanes + S::O_COL;
+  bool ok = true;
+  // `ref` is what the exponents are relative to, in the log2 domain.  It follows the row's maximum
+  // only when that has grown by more than 2^8: the sums in tensor memory then have to be
+  // rescaled, which hardly ever happens after the first tiles.
+  float ref = -INFINITY, sum = 0.0f;
+  const uint32_t end = u + x.n, mine = u + ((u ^ team) & 1u);
+  for (uint32_t i = mine; i < end && ok; i += 2) {
+    // S of this tile, and P V of the team's tile before: P may be written, the sums be rescaled
+    if (!mbar_wait(base + S::S_FULL + team * 8, (i >> 1) & 1u) ||
+        (i > mine && !mbar_wait(base + S::O_FULL + team * 8, ((i >> 1) - 1) & 1u))) {
+      k7_raise(p.status, TOME_DEV_TIMEOUT);
+      ok = false;
     }
-    named_bar_sync(1, K7_SOFTMAX_WARPS * 32);
-    const int rows = min(8, x.rows - 8 * r);
-    for (int i = warp * 32 + lane; i < rows * (D / 2); i += K7_SOFTMAX_WARPS * 32) {
-      const int row = i / (D / 2), f = i - row * (D / 2);
-      float2 w[K7_SOFTMAX_WARPS];
-      float top = -INFINITY;
+    __syncwarp();
+    if (active) {
+      tc_fence_after_sync();
+      uint32_t s0[32], s1[32];
+      tmem_ld32(tmem + lanes + team * K7_KEYS, s0);
+      tmem_ld32(tmem + lanes + team * K7_KEYS + 32, s1);
+      tmem_ld_wait_dep(s0);
+      tmem_ld_wait_dep(s1);
+      const int32_t valid = x.len - (x.tile + static_cast<int32_t>(i - u)) * K7_KEYS;
+      if (valid < K7_KEYS) {
 #pragma unroll
-      for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
-        w[k] = ml[k * 8 + row];
-        top = fmaxf(top, w[k].x);
+        for (int k = 0; k < 32; ++k) {
+          if (k >= valid) s0[k] = 0xff800000u;
+          if (k + 32 >= valid) s1[k] = 0xff800000u;
+        }
       }
-      float2 v = make_float2(0.0f, 0.0f);
-      float l = 0.0f;
+      float big[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int k = 0; k < K7_SOFTMAX_WARPS; ++k) {
-        // a warp without a finite score has the weight 0, or 1 where it holds a NaN
-        const float a = w[k].x == -INFINITY ? (w[k].y == 0.0f ? 0.0f : 1.0f) : ex2f(w[k].x - top);
-        const float2 q = area[(k * 8 + row) * (D / 2) + (f ^ (row << 2))];
-        v.x = fmaf(a, q.x, v.x);
-        v.y = fmaf(a, q.y, v.y);
-        l = fmaf(a, w[k].y, l);
+      for (int k = 0; k < 32; ++k)
+        big[k & 3] = fmax3(big[k & 3], __uint_as_float(s0[k]), __uint_as_float(s1[k]));
+      const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * p.c;
+      // (lanes beyond the rows hold whatever the last piece left)
+      const bool grow = row < x.rows && (top > ref + 8.0f || (i == mine && top > ref));
+      if (__any_sync(0xffffffffu, grow)) {
+        const float next = grow ? top : ref;
+        const float alpha = next == -INFINITY ? 1.0f : ex2f(ref - next);
+        sum *= alpha;
+        ref = next;
+        if (i > mine) {
+#pragma unroll 1
+          for (int h = 0; h < D; h += 32) {
+            uint32_t r[32];
+            tmem_ld32(o_addr + team * D + h, r);
+            tmem_ld_wait_dep(r);
+#pragma unroll
+            for (int k = 0; k < 32; ++k) r[k] = __float_as_uint(__uint_as_float(r[k]) * alpha);
+            tmem_st32(o_addr + team * D + h, r);
+          }
+        }
       }
-      *reinterpret_cast<float2*>(out_o + (8 * r + row) * D + 2 * f) = v;
-      if (f == 0) out_ml[8 * r + row] = make_float2(top, l);
+      // a row that has seen nothing but -inf takes 0 as its reference: all its p are 0
+      const float off = ref == -INFINITY ? 0.0f : -ref;
+      const float2 c2 = make_float2(p.c, p.c), off2 = make_float2(off, off);
+      float2 la = make_float2(0.0f, 0.0f), lb = la;
+      uint32_t pw[32];
+#pragma unroll
+      for (int k = 0; k < 32; ++k) {  // two keys
+        float2 e = k < 16 ? make_float2(__uint_as_float(s0[2 * k]), __uint_as_float(s0[2 * k + 1]))
+                          : make_float2(__uint_as_float(s1[2 * k - 32]), __uint_as_float(s1[2 * k - 31]));
+        e = __ffma2_rn(e, c2, off2);
+        e.x = ex2f(e.x);
+        e.y = ex2f(e.y);
+        if (k & 1) la = __fadd2_rn(la, e);
+        else lb = __fadd2_rn(lb, e);
+        pw[k] = k7_pack(e.x, e.y, T());
+      }
+      tmem_st32(tmem + lanes + S::P_COL + team * (K7_KEYS / 2), pw);
+      sum += (la.x + la.y) + (lb.x + lb.y);
+      tmem_st_wait();
+      tc_fence_before_sync();
     }
-    named_bar_sync(1, K7_SOFTMAX_WARPS * 32);  // the space may be written again
+    __syncwarp();
+    if (lane == 0) mbar_arrive(base + S::P_FULL + team * 8);
   }
+  // The teams' sums meet: each team brings the rows' reference and sum, then writes half of the
+  // columns from both teams' O.
+  float2* const ml = reinterpret_cast<float2*>(smem + S::MEET_ML);
+  if (mine < end && ok) {
+    const uint32_t i = end - 1 - ((end - 1 - mine) & 1u);  // the team's last tile
+    if (!mbar_wait(base + S::O_FULL + team * 8, (i >> 1) & 1u)) {
+      k7_raise(p.status, TOME_DEV_TIMEOUT);
+      ok = false;
+    }
+    __syncwarp();
+    tc_fence_after_sync();
+  }
+  u = end;
+  ml[team * K7_ROWS + row] = make_float2(ref, sum);
+  tc_fence_before_sync();
+  k7_meet(p, base + S::MEET, met, lane, ok);
+  tc_fence_after_sync();
+  if (active) {
+    const float2 a = ml[row], b = ml[K7_ROWS + row];
+    const float top = fmaxf(a.x, b.x);
+    // a team without a finite score has the weight 0 (also one without a tile, whose O is
+    // another piece's), or 1 where it holds a NaN
+    const float wa = a.x == -INFINITY ? (a.y == 0.0f ? 0.0f : 1.0f) : ex2f(a.x - top);
+    const float wb = b.x == -INFINITY ? (b.y == 0.0f ? 0.0f : 1.0f) : ex2f(b.x - top);
+    float* dst = out_o + row * D + team * (D / 2);
+#pragma unroll 1
+    for (int h = 0; h < D / 2; h += 32) {
+      uint32_t ra[32], rb[32];
+      tmem_ld32(o_addr + team * (D / 2) + h, ra);
+      tmem_ld32(o_addr + D + team * (D / 2) + h, rb);
+      tmem_ld_wait_dep(ra);
+      tmem_ld_wait_dep(rb);
+      if (row < x.rows) {
+#pragma unroll
+        for (int k = 0; k < 32; ++k) {
+          const float va = wa == 0.0f ? 0.0f : __uint_as_float(ra[k]) * wa;
+          ra[k] = __float_as_uint(wb == 0.0f ? va : fmaf(__uint_as_float(rb[k]), wb, va));
+        }
+#pragma unroll
+        for (int k = 0; k < 32; k += 4) stg128(dst + h + k, make_uint4(ra[k], ra[k + 1], ra[k + 2], ra[k + 3]));
+      }
+    }
+    if (team == 0 && row < x.rows) out_ml[row] = make_float2(top, fmaf(wa, a.y, wb * b.y));
+  }
+  tc_fence_before_sync();
+  k7_meet(p, base + S::MEET, met, lane, ok);  // O, and the space of the exchange, may be written again
   return ok;
 }
 
+// Pipeline of the big items: two warps copy keys and values (16-byte asynchronous copies: pages of
+// any size, rows past the end filled with zeros) into a ring of four stages; one thread issues
+// S = Q K^T (128 x 64 x D) and another O = P V (128 x D x 64), with P read from tensor memory and O
+// added up there (a single thread's issue, 60 clocks per product, bound the kernel: 1700 clocks
+// per tile); two teams of four softmax warps take the tiles in turn, a row per thread, each with
+// its own running maximum, sum and O, which meet at the end of a piece.
 template <typename T, int D>
 __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Params p) {
   using S = K7Smem<D>;
@@ -571,477 +886,326 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
   K7Plan pl;
   pl.group = reinterpret_cast<int32_t*>(smem + S::PLAN);
   pl.block = pl.group + p.n_groups + 1;
-  pl.prefix = pl.block + p.n_groups + 1;
-  pl.suffix = pl.prefix + p.n_groups + 1;
-
+  pl.prefix[0] = pl.block + p.n_groups + 1;
+  pl.prefix[1] = pl.prefix[0] + p.n_groups + 1;
+  pl.suffix = pl.prefix[1] + p.n_groups + 1;
   K7Card* const cards = reinterpret_cast<K7Card*>(smem + S::CARDS);
 
-  if (threadIdx.x == K7_MMA_WARP * 32) {
+  if (threadIdx.x == K7_QK_WARP * 32) {
     for (int i = 0; i < K7_STAGES; ++i) {
       mbar_init(base + S::FULL + i * 8, K7_COPY_THREADS);
-      mbar_init(base + S::EMPTY + i * 8, K7_SOFTMAX_WARPS);
+      mbar_init(base + S::EMPTY + i * 8, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(base + S::S_FULL + i * 8, 1);
-      mbar_init(base + S::P_FULL + i * 8, K7_SOFTMAX_WARPS);
+      mbar_init(base + S::P_FULL + i * 8, K7_TEAM_WARPS);
       mbar_init(base + S::O_FULL + i * 8, 1);
-      mbar_init(base + S::Q_EMPTY + i * 8, K7_SOFTMAX_WARPS);
+      mbar_init(base + S::Q_EMPTY + i * 8, 1);
     }
+    mbar_init(base + S::MEET, K7_SOFTMAX_WARPS);
     for (int i = 0; i < K7_CARDS; ++i) mbar_init(base + S::CARD_FULL + i * 8, 1);
     fence_mbar_init();
   }
-  if (warp == K7_MMA_WARP) {
-    __syncwarp();
-    tmem_alloc(base + S::TMEM, S::TMEM_COLS);
-    tmem_relinquish();
-  }
-  k7_build_plan(p, pl, warp, lane);
-  tc_fence_before_sync();
-  __syncthreads();
-  tc_fence_after_sync();
-  const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + S::TMEM);
-  const int32_t cost = pl.prefix[p.n_groups] + pl.suffix[p.n_seq];
-  const int32_t working = k7_working(cost, p.ctas);
-  const bool works = static_cast<int32_t>(blockIdx.x) < working;
-  const int32_t first = works ? k7_begin(cost, working, blockIdx.x) : 0;
-  const int32_t last = works ? k7_begin(cost, working, blockIdx.x + 1) : 0;
+  griddep_wait();  // what the kernels before write is read from here on
   griddep_launch_dependents();
+  k7_build_plan(p, pl, warp, lane);
+  __syncthreads();
+  const K7Split big(k7_cost(p, pl, true), p.ctas, p.inv_ctas, true);
+  const K7Split small(k7_cost(p, pl, false), p.ctas * K7_WARPS, p.inv_ctas / K7_WARPS, false);
 
-  if (warp < K7_SOFTMAX_WARPS) {
-    // ------------------------------------------------------------ softmax: thread = row
-    const int row = threadIdx.x;
-    const uint32_t lanes = static_cast<uint32_t>(warp * 32) << 16;
-    // counts of tiles (the ring), of tiles and pieces on the tensor core, of all pieces
-    uint32_t t = 0, u = 0, big_piece = 0, piece = 0;
-    bool ok = true;
-    // For the joining kernel, dealt over the CTAs: where a sequence's items lie.
-    for (int b = blockIdx.x * K7_SOFTMAX_WARPS * 32 + threadIdx.x; b < p.n_seq;
-         b += gridDim.x * K7_SOFTMAX_WARPS * 32) {
-      int4 a = make_int4(0, 0, 0, 0);  // its row within the group, the group's first row block and place, tiles
-      int32_t prefix_tile = K7_SMALL_COST;
-      if (p.n_groups > 0 && b >= pl.group[0] && b < pl.group[p.n_groups]) {
-        const int g = k7_find(pl.group, p.n_groups, b);
-        a = make_int4((b - pl.group[g]) * p.ratio, pl.block[g], pl.prefix[g],
-                      k7_tiles(k7_length(p, p.prefix_lens[g], p.prefix_blocks)));
-        prefix_tile = k7_tile_cost((pl.group[g + 1] - pl.group[g]) * p.ratio);
-        if (p.prefix_lens[g] > static_cast<int64_t>(p.prefix_blocks) * p.block_size)
-          k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);
-      }
-      const int32_t len = k7_length(p, p.lengths[b], p.seq_blocks);
-      if (p.lengths[b] > len) k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);
-      reinterpret_cast<int4*>(p.plan + 4)[2 * b] = a;
-      reinterpret_cast<int4*>(p.plan + 4)[2 * b + 1] =
-          make_int4(pl.prefix[p.n_groups] + pl.suffix[b], k7_tiles(len), prefix_tile, k7_tile_cost(p.ratio));
+  if (big.cost > 0) {  // (the same for all threads of all CTAs)
+    if (warp == K7_QK_WARP) {
+      tmem_alloc(base + S::TMEM, S::TMEM_COLS);
+      tmem_relinquish();
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) p.plan[0] = cost;
-
-    for (; ok; ++piece) {
-      if (!mbar_wait(base + S::CARD_FULL + (piece % K7_CARDS) * 8, (piece / K7_CARDS) & 1u)) {
-        k7_raise(p.status, TOME_DEV_TIMEOUT);
-        break;
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    const uint32_t tmem = *reinterpret_cast<volatile uint32_t*>(smem + S::TMEM);
+    const bool works = static_cast<int32_t>(blockIdx.x) < big.workers;
+    const int32_t first = works ? big.begin(blockIdx.x) : 0;
+    const int32_t last = works ? big.begin(blockIdx.x + 1) : 0;
+    if (warp < K7_SOFTMAX_WARPS) {
+      // ---------------------------------------------------------- softmax
+      uint32_t u = 0, piece = 0, met = 0;  // tiles, pieces, meetings so far; a tile's team is its parity
+      for (bool ok = true; ok; ++piece) {
+        if (!mbar_wait(base + S::CARD_FULL + (piece % K7_CARDS) * 8, (piece / K7_CARDS) & 1u)) {
+          k7_raise(p.status, TOME_DEV_TIMEOUT);
+          break;
+        }
+        const K7Card x = cards[piece % K7_CARDS];
+        if (x.n == 0) break;
+        const int64_t out_row = k7_out_row(p, x.prefix != 0, true, x.item, blockIdx.x);
+        ok = k7_big_piece<T, D>(p, smem, base, tmem, x, u, warp, lane, p.part_o + out_row * D, p.part_ml + out_row, met);
       }
-      const K7Card x = cards[piece % K7_CARDS];
-      if (x.n == 0) break;
-      const int64_t slot = static_cast<int64_t>(x.item) + blockIdx.x;
-      const int64_t rows_at = x.prefix ? slot * K7_ROWS : slot * p.ratio;
-      float* const out_o = (x.prefix ? p.prefix_o : p.suffix_o) + rows_at * D;
-      float2* const out_ml = (x.prefix ? p.prefix_ml : p.suffix_ml) + rows_at;
-      if (x.rows <= K7_SMALL_ROWS) {
-        ok = k7_small_piece<T, D>(p, smem, base, x, t, piece, warp, lane, out_o, out_ml);
-        continue;
+    } else if (warp == K7_QK_WARP) {
+      // ---------------------------------------------------------- tensor-core products
+      if (lane == 0) {
+        const uint64_t q_desc = k7_desc_k(base + S::Q), k_desc = k7_desc_k(base + S::KV);
+        uint32_t u = 0, piece = 0;
+        bool ok = true;
+        K7Piece x;
+        int32_t at = first;
+        for (; ok && k7_next<true>(p, pl, x, piece > 0, at, last); ++piece) {
+          for (int32_t j = 0; j < x.n; ++j, ++u) {
+            const uint32_t stage = u % K7_STAGES, team = u & 1u;
+            // keys (and queries) are there, and the team has read the scores that lie where these go
+            if (!mbar_wait(base + S::FULL + stage * 8, (u / K7_STAGES) & 1u) ||
+                (u >= 2 && !mbar_wait(base + S::P_FULL + team * 8, ((u >> 1) - 1) & 1u))) {
+              k7_raise(p.status, TOME_DEV_TIMEOUT);
+              ok = false;
+              break;
+            }
+            fence_proxy_async();  // the copies are ordinary writes: visible to the tensor core from here
+            tc_fence_after_sync();
+            const uint64_t a = q_desc + (piece & 1u) * (S::Q_BYTES >> 4), b = k_desc + stage * (S::STAGE >> 4);
+#pragma unroll
+            for (int k = 0; k < D / 16; ++k)
+              umma_bf16_ss(tmem + team * K7_KEYS, a + (k / 4) * (K7_ROWS * 128 >> 4) + 2 * (k % 4),
+                           b + (k / 4) * (K7_KEYS * 128 >> 4) + 2 * (k % 4), k7_idesc<T>(K7_KEYS, false), k != 0);
+            umma_commit(base + S::S_FULL + team * 8);
+            if (j == x.n - 1) umma_commit(base + S::Q_EMPTY + (piece & 1u) * 8);
+          }
+        }
       }
-      const bool active = warp * 32 < x.rows;  // warps without a row only keep step
-      const uint32_t o_addr = tmem + lanes + 2 * K7_KEYS + (big_piece & 1u) * D;
-      // `ref` is what the exponents are relative to, in the log2 domain.  It follows the row's
-      // maximum only when that has grown by more than 2^8: the sums in tensor memory then
-      // have to be rescaled, which hardly ever happens after the first tiles.
-      float ref = -INFINITY, sum = 0.0f;
-      for (int32_t j = 0; j < x.n && ok; ++j, ++t, ++u) {
-        const uint32_t buf = u & 1u;
-        if (!mbar_wait(base + S::S_FULL + buf * 8, (u >> 1) & 1u)) {
+      __syncwarp();
+    } else if (warp == K7_PV_WARP) {
+      if (lane == 0) {
+        const uint64_t v_desc = k7_desc_mn(base + S::KV + S::KV_BYTES, K7_KEYS * 128);
+        uint32_t u = 0, piece = 0;
+        bool ok = true;
+        K7Piece x;
+        int32_t at = first;
+        for (; ok && k7_next<true>(p, pl, x, piece > 0, at, last); ++piece) {
+          for (int32_t j = 0; j < x.n; ++j, ++u) {
+            const uint32_t stage = u % K7_STAGES, team = u & 1u;
+            if (!mbar_wait(base + S::P_FULL + team * 8, (u >> 1) & 1u) ||
+                !mbar_wait(base + S::FULL + stage * 8, (u / K7_STAGES) & 1u)) {  // (done long ago)
+              k7_raise(p.status, TOME_DEV_TIMEOUT);
+              ok = false;
+              break;
+            }
+            fence_proxy_async();
+            tc_fence_after_sync();
+            const uint64_t b = v_desc + stage * (S::STAGE >> 4);
+            const uint32_t d = tmem + S::O_COL + team * D, a = tmem + S::P_COL + team * (K7_KEYS / 2);
+#pragma unroll
+            for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 8 columns of P, 16 rows of V
+              umma_f16_ts(d, a + 8 * k, b + (2048 >> 4) * k, k7_idesc<T>(D, true), j > 1 || k != 0);
+            umma_commit(base + S::EMPTY + stage * 8);
+            umma_commit(base + S::O_FULL + team * 8);
+          }
+        }
+        // nothing may still be under way when the space is used otherwise
+        for (uint32_t i = u > 2 ? u - 2 : 0; i < u && ok; ++i)
+          if (!mbar_wait(base + S::O_FULL + (i & 1u) * 8, (i >> 1) & 1u)) {
+            k7_raise(p.status, TOME_DEV_TIMEOUT);
+            ok = false;
+          }
+      }
+      __syncwarp();
+    } else if (warp < K7_PV_WARP) {
+      // ---------------------------------------------------------- copies
+      constexpr int PIECES = D / 8;                  // 16-byte pieces of a row
+      constexpr int AT_ONCE = 32 / PIECES;           // rows that a warp copies per step
+      constexpr int STEPS = 32 / AT_ONCE;            // a warp has 32 of the 64 keys
+      const int cw = warp - (K7_QK_WARP + 1);
+      const int c = lane % PIECES, sub = lane / PIECES;
+      const int my_row = cw * 32;
+      const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
+      const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
+      const uint32_t area = base + S::KV + (c >> 3) * (K7_KEYS * 128);
+      auto show = [&](const K7Piece& y, uint32_t index, bool there) {  // to the softmax warps
+        if (cw == 0 && lane == 0) {
+          cards[index % K7_CARDS] = K7Card{y.len, y.tile, there ? y.n : 0, y.rows, y.item, y.prefix ? 1 : 0};
+          mbar_arrive(base + S::CARD_FULL + (index % K7_CARDS) * 8);
+        }
+      };
+      uint32_t t = 0, piece = 0;
+      bool ok = true;
+      int32_t at = first;
+      K7Piece x = {};
+      K7Pages pages = {};
+      bool there = k7_next<true>(p, pl, x, false, at, last);
+      show(x, 0, there);
+      if (there) pages = k7_open_pages(p, x, x.tile * K7_KEYS + my_row, lane);
+      while (there && ok) {
+        if (piece >= 2 && !mbar_wait(base + S::Q_EMPTY + (piece & 1u) * 8, ((piece >> 1) - 1) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
           ok = false;
           break;
         }
-        __syncwarp();
-        if (active) {
-          tc_fence_after_sync();
-          uint32_t s0[32], s1[32];
-          tmem_ld32(tmem + lanes + buf * K7_KEYS, s0);
-          tmem_ld32(tmem + lanes + buf * K7_KEYS + 32, s1);
-          tmem_ld_wait_dep(s0);
-          tmem_ld_wait_dep(s1);
-          const int32_t valid = x.len - (x.tile + j) * K7_KEYS;
-          if (valid < K7_KEYS) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) {
-              if (i >= valid) s0[i] = 0xff800000u;
-              if (i + 32 >= valid) s1[i] = 0xff800000u;
-            }
-          }
-          float big[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            big[i & 3] = fmax3(big[i & 3], __uint_as_float(s0[i]), __uint_as_float(s1[i]));
-          const float top = fmaxf(fmaxf(big[0], big[1]), fmaxf(big[2], big[3])) * p.c;
-          // (lanes beyond the rows hold whatever the last piece left)
-          const bool grow = row < x.rows && (top > ref + 8.0f || (j == 0 && top > ref));
-          // P V of the tile before is done: P may be written again, and the sums be rescaled
-          if (j > 0) {
-            if (!mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u)) {
-              k7_raise(p.status, TOME_DEV_TIMEOUT);
-              ok = false;
-            }
-            __syncwarp();
-          }
-          if (__any_sync(0xffffffffu, grow)) {
-            const float next = grow ? top : ref;
-            const float alpha = next == -INFINITY ? 1.0f : ex2f(ref - next);
-            sum *= alpha;
-            ref = next;
-            if (j > 0) {
-              tc_fence_after_sync();
-#pragma unroll 1
-              for (int h = 0; h < D; h += 32) {
-                uint32_t r[32];
-                tmem_ld32(o_addr + h, r);
-                tmem_ld_wait_dep(r);
-#pragma unroll
-                for (int i = 0; i < 32; ++i) r[i] = __float_as_uint(__uint_as_float(r[i]) * alpha);
-                tmem_st32(o_addr + h, r);
-              }
-              tmem_st_wait();
-            }
-          }
-          // a row that has seen nothing but -inf takes 0 as its reference: all its p are 0
-          const float off = ref == -INFINITY ? 0.0f : -ref;
-          const float2 c2 = make_float2(p.c, p.c), off2 = make_float2(off, off);
-          float2 la = make_float2(0.0f, 0.0f), lb = la;
-          const uint32_t prow = base + S::P + row * 128;
-#pragma unroll
-          for (int h = 0; h < 8; ++h) {  // eight keys: one 16-byte piece of P
-            float2 e[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int w = (h & 3) * 8 + 2 * i;
-              e[i] = h < 4 ? make_float2(__uint_as_float(s0[w]), __uint_as_float(s0[w + 1]))
-                           : make_float2(__uint_as_float(s1[w]), __uint_as_float(s1[w + 1]));
-              e[i] = __ffma2_rn(e[i], c2, off2);
-              e[i].x = ex2f(e[i].x);
-              e[i].y = ex2f(e[i].y);
-            }
-            la = __fadd2_rn(la, __fadd2_rn(e[0], e[1]));
-            lb = __fadd2_rn(lb, __fadd2_rn(e[2], e[3]));
-            k7_sts128(prow + ((h ^ (row & 7)) << 4),
-                      make_uint4(k7_pack(e[0].x, e[0].y, T()), k7_pack(e[1].x, e[1].y, T()),
-                                 k7_pack(e[2].x, e[2].y, T()), k7_pack(e[3].x, e[3].y, T())));
-          }
-          sum += (la.x + la.y) + (lb.x + lb.y);
-          fence_proxy_async();
-          tc_fence_before_sync();
+        for (int i = cw * AT_ONCE + sub; i < x.rows; i += 2 * AT_ONCE) {
+          const int32_t row = x.row0 + i, s = row / p.ratio;
+          const T* src = reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
+                         static_cast<int64_t>(x.kv_head * p.ratio + (row - s * p.ratio)) * D + c * 8;
+          k7_copy16(base + S::Q + (piece & 1u) * S::Q_BYTES + (c >> 3) * (K7_ROWS * 128) + i * 128 +
+                        (((c & 7) ^ (i & 7)) << 4),
+                    src, true);
         }
-        __syncwarp();
-        if (lane == 0) mbar_arrive(base + S::P_FULL + buf * 8);
-      }
-      ++big_piece;
-      // (warps without a row wait too: what follows may write where the products read P)
-      if (ok && !mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u)) {
-        k7_raise(p.status, TOME_DEV_TIMEOUT);
-        ok = false;
-      }
-      if (!active || !ok) continue;
-      __syncwarp();
-      tc_fence_after_sync();
-      float* dst = out_o + row * D;
-#pragma unroll 1
-      for (int h = 0; h < D; h += 32) {
-        uint32_t r[32];
-        tmem_ld32(o_addr + h, r);
-        tmem_ld_wait_dep(r);
-        if (row < x.rows) {
-#pragma unroll
-          for (int i = 0; i < 32; i += 4)
-            stg128(dst + h + i, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]));
-        }
-      }
-      tc_fence_before_sync();
-      if (row < x.rows) out_ml[row] = make_float2(ref, sum);
-    }
-  } else if (warp == K7_MMA_WARP) {
-    // ------------------------------------------------------------ tensor-core products
-    if (lane == 0) {
-      // counts as above; the product P V of a tile is issued after Q K of the next one
-      uint32_t t = 0, u = 0, big_piece = 0, piece = 0;
-      bool ok = true, pending = false, pending_add = false;
-      uint32_t pending_stage = 0, pending_o = 0;
-      auto multiply_pv = [&]() {  // O (+)= P V of tile u - 1
-        pending = false;
-        const uint32_t buf = (u - 1) & 1u;
-        if (!mbar_wait(base + S::P_FULL + buf * 8, ((u - 1) >> 1) & 1u)) {
-          k7_raise(p.status, TOME_DEV_TIMEOUT);
-          ok = false;
-          return;
-        }
-        tc_fence_after_sync();
-        const uint64_t a = k7_desc_k(base + S::P);
-        const uint64_t b = k7_desc_mn(base + S::KV + pending_stage * S::STAGE + S::KV_BYTES, K7_KEYS * 128);
-#pragma unroll
-        for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 32 bytes of a P row, 16 rows of V
-          umma_bf16_ss(tmem + 2 * K7_KEYS + pending_o * D, a + 2 * k, b + (2048 >> 4) * k,
-                       k7_idesc<T>(D, true), pending_add || k != 0);
-        // a stage is given back by four arrivals (of four warps, where those do the products)
-        for (int i = 1; i < K7_SOFTMAX_WARPS; ++i) mbar_arrive(base + S::EMPTY + pending_stage * 8);
-        umma_commit(base + S::EMPTY + pending_stage * 8);
-        umma_commit(base + S::O_FULL + buf * 8);
-      };
-      K7Piece x;
-      int32_t at = first;
-      for (; ok && k7_next(p, pl, x, piece > 0, at, last); ++piece) {
-        if (x.rows <= K7_SMALL_ROWS) {
-          if (pending) multiply_pv();
-          t += x.n;
-          continue;
-        }
-        for (int32_t j = 0; j < x.n && ok; ++j, ++t) {
+        K7Piece next = x;
+        K7Pages next_pages = {};
+        bool next_there = false;
+        for (int32_t j = 0; j < x.n; ++j, ++t) {
           const uint32_t stage = t % K7_STAGES;
-          if (!mbar_wait(base + S::FULL + stage * 8, (t / K7_STAGES) & 1u)) {
+          if (j + 1 == x.n) {  // the piece behind is looked up while this one's loads are under way
+            next_there = k7_next<true>(p, pl, next, true, at, last);
+            show(next, piece + 1, next_there);
+            if (next_there) next_pages = k7_open_pages(p, next, next.tile * K7_KEYS + my_row, lane);
+          }
+          if (t >= K7_STAGES && !mbar_wait(base + S::EMPTY + stage * 8, (t / K7_STAGES - 1) & 1u)) {
             k7_raise(p.status, TOME_DEV_TIMEOUT);
             ok = false;
             break;
           }
-          fence_proxy_async();  // the copies are ordinary writes: visible to the tensor core from here
-          tc_fence_after_sync();
+          __syncwarp();
+          const int32_t pool_row = k7_pool_row(p, x, pages, (x.tile + j) * K7_KEYS + my_row, lane);
+          const uint32_t dst = area + stage * S::STAGE;
 #pragma unroll
-          for (int k = 0; k < D / 16; ++k) {
-            const uint64_t a = k7_desc_k(base + S::Q + (piece & 1u) * S::Q_BYTES + (k / 4) * (K7_ROWS * 128)) + 2 * (k % 4);
-            const uint64_t b = k7_desc_k(base + S::KV + stage * S::STAGE + (k / 4) * (K7_KEYS * 128)) + 2 * (k % 4);
-            umma_bf16_ss(tmem + (u & 1u) * K7_KEYS, a, b, k7_idesc<T>(K7_KEYS, false), k != 0);
+          for (int i = 0; i < STEPS; ++i) {
+            const int r = my_row + i * AT_ONCE + sub;
+            const int32_t from = __shfl_sync(0xffffffffu, pool_row, i * AT_ONCE + sub);
+            const int64_t off = static_cast<int64_t>(max(from, 0)) * D;
+            const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+            k7_copy16(to, k_pool + off, from >= 0);
+            k7_copy16(to + S::KV_BYTES, v_pool + off, from >= 0);
           }
-          umma_commit(base + S::S_FULL + (u & 1u) * 8);
-          if (j == x.n - 1) {
-            for (int i = 1; i < K7_SOFTMAX_WARPS; ++i) mbar_arrive(base + S::Q_EMPTY + (piece & 1u) * 8);
-            umma_commit(base + S::Q_EMPTY + (piece & 1u) * 8);
-          }
-          if (pending) multiply_pv();
-          pending = true;
-          pending_add = j > 0;
-          pending_stage = stage;
-          pending_o = big_piece & 1u;
-          ++u;
+          k7_copies_arrive(base + S::FULL + stage * 8);
         }
-        ++big_piece;
+        x = next;
+        pages = next_pages;
+        there = next_there;
+        ++piece;
       }
-      if (ok && pending) multiply_pv();
-      // nothing may still be under way when the block leaves
-      if (ok && u > 0 && !mbar_wait(base + S::O_FULL + ((u - 1) & 1u) * 8, ((u - 1) >> 1) & 1u))
-        k7_raise(p.status, TOME_DEV_TIMEOUT);
+      asm volatile("cp.async.wait_all;" ::: "memory");
     }
-    __syncwarp();
-  } else {
-    // ------------------------------------------------------------ copies
-    constexpr int PIECES = D / 8;                  // 16-byte pieces of a row
-    constexpr int AT_ONCE = 32 / PIECES;           // rows that a warp copies per step
-    constexpr int STEPS = 32 / AT_ONCE;            // a warp has 32 of the 64 keys
-    const int cw = warp - (K7_MMA_WARP + 1);
-    const int c = lane % PIECES, sub = lane / PIECES;
-    const int my_row = cw * 32;
-    const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
-    const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
-    const uint32_t area = base + S::KV + (c >> 3) * (K7_KEYS * 128);
-    auto block_of = [&](int32_t key) {
-      return static_cast<int32_t>(static_cast<uint64_t>(key) * p.div_magic >> p.div_shift);
-    };
-    // 64 entries of the table from block `first` on, two per lane: a tile's pages come from there by
-    // shuffles, and the entries behind them are asked for long before they are needed.
-    struct Pages {
-      int32_t first, a, b;
-    };
-    auto ask = [&](const K7Piece& y, int32_t block) {
-      return block <= block_of(y.len - 1) ? __ldg(y.table + block) : -1;
-    };
-    auto open_pages = [&](const K7Piece& y) {
-      const int32_t f = block_of(min(y.tile * K7_KEYS + my_row, y.len - 1));
-      return Pages{f, ask(y, f + lane), ask(y, f + 32 + lane)};
-    };
-    // The pool's row (blocks and heads flattened) of key (tile * 64 + my_row + lane), or -1.
-    auto pool_row_of = [&](const K7Piece& y, Pages& w, int32_t tile) -> int32_t {
-      const int32_t key0 = tile * K7_KEYS + my_row, key = key0 + lane;
-      if (key0 >= y.len) return -1;
-      const int32_t lo = block_of(key0);
-      if (lo - w.first >= 32) {
-        if (lo - w.first < 64) w = Pages{w.first + 32, w.b, ask(y, w.first + 64 + lane)};
-        else w = Pages{lo, ask(y, lo + lane), ask(y, lo + 32 + lane)};
-      }
-      const int32_t blk = block_of(min(key, y.len - 1)), rel = blk - w.first;  // 0 .. 62
-      const int32_t pa = __shfl_sync(0xffffffffu, w.a, rel & 31), pb = __shfl_sync(0xffffffffu, w.b, rel & 31);
-      const int32_t page = rel < 32 ? pa : pb;
-      if (key >= y.len) return -1;
-      if (page < 0 || page >= p.num_blocks) {
-        k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);  // reads as zeros, as gather does
-        return -1;
-      }
-      return (page * p.kv_heads + y.kv_head) * p.block_size + (key - blk * p.block_size);
-    };
-    auto show = [&](const K7Piece& y, uint32_t index, bool there) {  // to the softmax warps
-      if (cw == 0 && lane == 0) {
-        cards[index % K7_CARDS] = K7Card{y.len, y.tile, there ? y.n : 0, y.rows, y.item, y.prefix ? 1 : 0};
-        mbar_arrive(base + S::CARD_FULL + (index % K7_CARDS) * 8);
-      }
-    };
-    uint32_t t = 0, piece = 0;
-    bool ok = true;
-    int32_t at = first;
-    K7Piece x = {};
-    Pages pages = {};
-    bool there = k7_next(p, pl, x, false, at, last);
-    show(x, 0, there);
-    if (there) pages = open_pages(x);
-    while (there && ok) {
-      if (piece >= 2 && !mbar_wait(base + S::Q_EMPTY + (piece & 1u) * 8, ((piece >> 1) - 1) & 1u)) {
-        k7_raise(p.status, TOME_DEV_TIMEOUT);
-        ok = false;
-        break;
-      }
-      for (int i = cw * AT_ONCE + sub; i < x.rows; i += 2 * AT_ONCE) {
-        const int32_t row = x.row0 + i, s = row / p.ratio;
-        const T* src = reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
-                       static_cast<int64_t>(x.kv_head * p.ratio + (row - s * p.ratio)) * D + c * 8;
-        k7_copy16(base + S::Q + (piece & 1u) * S::Q_BYTES + (c >> 3) * (K7_ROWS * 128) + i * 128 +
-                      (((c & 7) ^ (i & 7)) << 4),
-                  src, true);
-      }
-      K7Piece next = x;
-      Pages next_pages = {};
-      bool next_there = false;
-      for (int32_t j = 0; j < x.n; ++j, ++t) {
-        const uint32_t stage = t % K7_STAGES;
-        if (j + 1 == x.n) {  // the piece behind is looked up while this one's loads are under way
-          next_there = k7_next(p, pl, next, true, at, last);
-          show(next, piece + 1, next_there);
-          if (next_there) next_pages = open_pages(next);
-        }
-        if (t >= K7_STAGES && !mbar_wait(base + S::EMPTY + stage * 8, (t / K7_STAGES - 1) & 1u)) {
-          k7_raise(p.status, TOME_DEV_TIMEOUT);
-          ok = false;
-          break;
-        }
-        __syncwarp();
-        const int32_t pool_row = pool_row_of(x, pages, x.tile + j);
-        const uint32_t dst = area + stage * S::STAGE;
-#pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          const int r = my_row + i * AT_ONCE + sub;
-          const int32_t from = __shfl_sync(0xffffffffu, pool_row, i * AT_ONCE + sub);
-          const int64_t off = static_cast<int64_t>(max(from, 0)) * D;
-          const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-          k7_copy16(to, k_pool + off, from >= 0);
-          k7_copy16(to + S::KV_BYTES, v_pool + off, from >= 0);
-        }
-        k7_copies_arrive(base + S::FULL + stage * 8);
-      }
-      x = next;
-      pages = next_pages;
-      there = next_there;
-      ++piece;
+    tc_fence_before_sync();
+    __syncthreads();
+    if (warp == K7_QK_WARP) {
+      tc_fence_after_sync();
+      tmem_dealloc(tmem, S::TMEM_COLS);
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   }
-  tc_fence_before_sync();
-  __syncthreads();
-  if (warp == K7_MMA_WARP) {
-    tc_fence_after_sync();
-    tmem_dealloc(tmem, S::TMEM_COLS);
+
+  if (warp == K7_PV_WARP) {
+    // For the joining kernel, dealt over the CTAs: where a row's pieces lie.
+    for (int64_t i = blockIdx.x * 32 + lane; i < static_cast<int64_t>(p.n_seq) * p.heads; i += gridDim.x * 32) {
+      const int32_t b = static_cast<int32_t>(i / p.heads), h = static_cast<int32_t>(i - static_cast<int64_t>(b) * p.heads);
+      const int32_t kv = h / p.ratio, hr = h - kv * p.ratio;
+      int4 where = make_int4(0, 0, 0, 0);
+      if (p.n_groups > 0 && b >= pl.group[0] && b < pl.group[p.n_groups]) {
+        const int g = k7_find(pl.group, p.n_groups, b);
+        const int32_t len = k7_length(p, p.prefix_lens[g], p.prefix_blocks);
+        const bool is_big = k7_is_big((pl.group[g + 1] - pl.group[g]) * p.ratio);
+        const int32_t row = (b - pl.group[g]) * p.ratio + hr, mb = is_big ? row / K7_ROWS : 0, in_group = mb * p.kv_heads + kv;
+        if (len > 0) {
+          const int2 w = k7_holders(is_big ? big : small, pl.prefix[is_big][g] + in_group * k7_item_cost(len, is_big), len, is_big);
+          const int32_t item = (is_big ? pl.block[g] : g) * p.kv_heads + in_group;
+          where.x = static_cast<int32_t>(k7_out_row(p, true, is_big, item, w.x)) + (row - mb * K7_ROWS);
+          where.y = is_big ? w.y : -w.y;
+        }
+        if (p.prefix_lens[g] > len) k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);
+      }
+      const int32_t len = k7_length(p, p.lengths[b], p.seq_blocks);
+      if (p.lengths[b] > len) k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);
+      if (len > 0) {
+        const bool is_big = k7_is_big(p.ratio);
+        const int2 w = k7_holders(is_big ? big : small,
+                                  pl.prefix[is_big][p.n_groups] + pl.suffix[b] + kv * k7_item_cost(len, is_big), len, is_big);
+        where.z = static_cast<int32_t>(k7_out_row(p, false, is_big, b * p.kv_heads + kv, w.x)) + hr;
+        where.w = w.y;
+      }
+      p.plan[i] = where;
+    }
   }
+  // the first workers are spread over the CTAs
+  const int32_t worker = warp * gridDim.x + blockIdx.x;
+  if (worker < small.workers)
+    k7_small_run<T, D>(p, pl, base + warp * (K7_SMALL_STAGES * S::SMALL_STAGE), worker, small.begin(worker),
+                       small.begin(worker + 1), lane);
 }
 
 // ------------------------------------------------------------------ joining the pieces
-// One warp per (sequence, head).  With maxima m_i, sums l_i and sums of p v o_i of its pieces:
-// M = max m_i, out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.  A row without a key is 0 with
-// log-sum -inf.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) k7_join_kernel(const K7Params p) {
-  constexpr int E = D / 32;  // elements per lane
-  const int lane = threadIdx.x & 31;
-  const int64_t w = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 5);
+// With maxima m_i, sums l_i and sums of p v o_i of a row's pieces: M = max m_i,
+// out = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i.  A row without a key is 0 with log-sum -inf.
+// WARPS warps share a row's pieces.  Little but the latency of two loads: where the pieces are,
+// then all of them at once.
+constexpr int K7_JOIN_WARPS = 4;
+
+template <typename T, int D, int WARPS>
+__global__ void __launch_bounds__(K7_JOIN_WARPS * 32) k7_join_kernel(const K7Params p) {
+  constexpr int E = D / 32;       // elements per lane
+  constexpr int TOGETHER = 8;     // pieces whose loads are under way at a time
+  __shared__ float part[WARPS][D];
+  __shared__ float2 part_ml[WARPS];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t w = WARPS > 1 ? static_cast<int64_t>(blockIdx.x)
+                              : static_cast<int64_t>(blockIdx.x) * K7_JOIN_WARPS + warp;
   griddep_wait();
-  if (w >= static_cast<int64_t>(p.n_seq) * p.heads) return;
-  const int32_t b = static_cast<int32_t>(w / p.heads), h = static_cast<int32_t>(w - static_cast<int64_t>(b) * p.heads);
-  const int32_t kv = h / p.ratio;
-  const int32_t cost = p.plan[0], working = k7_working(cost, p.ctas);
-  const int4 a = reinterpret_cast<const int4*>(p.plan + 4)[2 * b];
-  const int4 s = reinterpret_cast<const int4*>(p.plan + 4)[2 * b + 1];
-  const int32_t row = a.x + (h - kv * p.ratio), mb = row / K7_ROWS;
-  // the CTAs that hold parts of the row's two items, and the row's place in the first one's slot
-  int32_t n_prefix = 0, n_suffix = 0, prefix_cta = 0, suffix_cta = 0, prefix_begin = 0, suffix_begin = 0;
-  int64_t at_prefix = 0, at_suffix = 0;
-  const int32_t prefix_cost = k7_item_cost(a.w, s.z), suffix_cost = k7_item_cost(s.y, s.w);
-  if (a.w > 0) {
-    const int32_t i = mb * p.kv_heads + kv;
-    prefix_begin = a.z + i * prefix_cost;
-    prefix_cta = k7_cta_of(cost, working, prefix_begin);
-    n_prefix = k7_cta_of(cost, working, prefix_begin + prefix_cost - 1) - prefix_cta + 1;
-    at_prefix = (static_cast<int64_t>(a.y) * p.kv_heads + i + prefix_cta) * K7_ROWS + (row - mb * K7_ROWS);
-  }
-  if (s.y > 0) {
-    suffix_begin = s.x + kv * suffix_cost;
-    suffix_cta = k7_cta_of(cost, working, suffix_begin);
-    n_suffix = k7_cta_of(cost, working, suffix_begin + suffix_cost - 1) - suffix_cta + 1;
-    at_suffix = (static_cast<int64_t>(b) * p.kv_heads + kv + suffix_cta) * p.ratio + (h - kv * p.ratio);
-  }
-  const int32_t n = n_prefix + n_suffix;
+  griddep_launch_dependents();
+  if (w >= static_cast<int64_t>(p.n_seq) * p.heads) return;  // (never with WARPS > 1)
+  const int4 where = p.plan[w];
+  const int32_t n_prefix = abs(where.y), n = n_prefix + where.w;
+  const int32_t prefix_step = where.y < 0 ? K7_SMALL_ROWS : K7_ROWS;
   float top = -INFINITY, total = 0.0f, acc[E];
 #pragma unroll
   for (int e = 0; e < E; ++e) acc[e] = 0.0f;
-  for (int32_t base = 0; base < n; base += 32) {
-    const int32_t i = base + lane;
-    float2 ml = make_float2(-INFINITY, 0.0f);
-    bool there = false;  // a CTA's run may hold less than a tile of the item
-    if (i < n) {
-      const bool pre = i < n_prefix;
-      const int32_t cta = pre ? prefix_cta + i : suffix_cta + i - n_prefix;
-      const int32_t begin = pre ? prefix_begin : suffix_begin, end = begin + (pre ? prefix_cost : suffix_cost);
-      const int32_t from = max(k7_begin(cost, working, cta), begin), to = min(k7_begin(cost, working, cta + 1), end);
-      const int32_t w1 = pre ? s.z : s.w;
-      there = k7_cut(to - begin, w1) > k7_cut(from - begin, w1);
-      if (there)
-        ml = pre ? p.prefix_ml[at_prefix + static_cast<int64_t>(i) * K7_ROWS]
-                 : p.suffix_ml[at_suffix + static_cast<int64_t>(i - n_prefix) * p.ratio];
-    }
-    if (ml.y == 0.0f) ml.x = -INFINITY;  // a piece that saw nothing but -inf
-    float m = ml.x;
+  // takes (m, l) and o of one more piece each; a sum of 0 is a piece that saw nothing but -inf, a
+  // maximum of -inf with a sum is one of NaN scores
+  auto take = [&](const float2 (&ml)[TOGETHER], const float (&v)[TOGETHER][E], int32_t count) {
+    float m = top;
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    m = fmaxf(m, top);
-    const float keep = top == -INFINITY ? 0.0f : ex2f(top - m);
+    for (int k = 0; k < TOGETHER; ++k)
+      if (k < count && ml[k].y != 0.0f) m = fmaxf(m, ml[k].x);
+    const float keep = top == -INFINITY ? (total == 0.0f ? 0.0f : 1.0f) : ex2f(top - m);
     top = m;
-    const float wgt = ml.x == -INFINITY ? 0.0f : ex2f(ml.x - m);
-    float l = wgt * ml.y;
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-    total = fmaf(total, keep, l);
+    total *= keep;
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[e] *= keep;
-    const uint32_t which = __ballot_sync(0xffffffffu, there);
-    const int32_t here = min(32, n - base);
-#pragma unroll 4
-    for (int32_t k = 0; k < here; ++k) {
-      const float f = __shfl_sync(0xffffffffu, wgt, k);
-      if (!(which >> k & 1u)) continue;
-      const int32_t q = base + k;
-      const float* src = q < n_prefix
-                             ? p.prefix_o + (at_prefix + static_cast<int64_t>(q) * K7_ROWS) * D
-                             : p.suffix_o + (at_suffix + static_cast<int64_t>(q - n_prefix) * p.ratio) * D;
-      float v[E];
-      if constexpr (E == 4) {
-        const float4 x = *reinterpret_cast<const float4*>(src + lane * 4);
-        v[0] = x.x; v[1] = x.y; v[2] = x.z; v[3] = x.w;
-      } else {
-        const float2 x = *reinterpret_cast<const float2*>(src + lane * 2);
-        v[0] = x.x; v[1] = x.y;
-      }
 #pragma unroll
-      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, v[e], acc[e]);
+    for (int k = 0; k < TOGETHER; ++k) {
+      if (k >= count || ml[k].y == 0.0f) continue;
+      const float f = ml[k].x == -INFINITY ? 1.0f : ex2f(ml[k].x - m);
+      total = fmaf(f, ml[k].y, total);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(f, v[k][e], acc[e]);
     }
+  };
+  for (int32_t base = WARPS > 1 ? warp * TOGETHER : 0; base < n; base += WARPS * TOGETHER) {
+    float v[TOGETHER][E];
+    float2 ml[TOGETHER];
+#pragma unroll
+    for (int k = 0; k < TOGETHER; ++k) {
+      const int32_t i = min(base + k, n - 1);
+      const int64_t row = i < n_prefix ? where.x + static_cast<int64_t>(i) * prefix_step
+                                       : where.z + static_cast<int64_t>(i - n_prefix) * p.ratio;
+      ml[k] = p.part_ml[row];
+      const float* src = p.part_o + row * D + lane * E;
+      if constexpr (E == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(src);
+        v[k][0] = x.x; v[k][1] = x.y; v[k][2] = x.z; v[k][3] = x.w;
+      } else {
+        const float2 x = *reinterpret_cast<const float2*>(src);
+        v[k][0] = x.x; v[k][1] = x.y;
+      }
+    }
+    take(ml, v, n - base);
+  }
+  if constexpr (WARPS > 1) {
+#pragma unroll
+    for (int e = 0; e < E; ++e) part[warp][lane * E + e] = acc[e];
+    if (lane == 0) part_ml[warp] = make_float2(top, total);
+    __syncthreads();
+    if (warp > 0) return;
+    float v[TOGETHER][E];
+    float2 ml[TOGETHER];
+#pragma unroll
+    for (int k = 1; k < WARPS; ++k) {
+      ml[k - 1] = part_ml[k];
+#pragma unroll
+      for (int e = 0; e < E; ++e) v[k - 1][e] = part[k][lane * E + e];
+    }
+    take(ml, v, WARPS - 1);
   }
   const float inv = total == 0.0f ? 0.0f : 1.0f / total;
   T* out = reinterpret_cast<T*>(p.out) + w * D + lane * E;
@@ -1056,28 +1220,24 @@ __global__ void __launch_bounds__(128) k7_join_kernel(const K7Params p) {
 
 // ------------------------------------------------------------------ host side
 struct K7Layout {
-  size_t plan, prefix_o, prefix_ml, suffix_o, suffix_ml, total;
+  int64_t small_rows, suffix_rows, rows;
+  size_t plan, part_o, part_ml, total;
 };
 
 static size_t k7_up(size_t n) { return (n + 255) / 256 * 256; }
-
-// The split takes at most this many CTAs (one per SM); the workspace does not depend on the
-// device that it is asked for on.
-constexpr int K7_MAX_CTAS = 160;
 
 static K7Layout k7_layout(int64_t n_seq, int64_t n_groups, int64_t heads, int64_t kv_heads, int64_t dim) {
   const int64_t ratio = heads / kv_heads;
   // row blocks of all groups: each group rounds up once
   const int64_t blocks = n_groups == 0 ? 0 : n_groups + n_seq * ratio / K7_ROWS;
-  const int64_t prefix_slots = blocks == 0 ? 0 : blocks * kv_heads + K7_MAX_CTAS;
-  const int64_t suffix_slots = n_seq * kv_heads + K7_MAX_CTAS;
   K7Layout l;
+  l.small_rows = n_groups == 0 ? 0 : (blocks * kv_heads + K7_MAX_CTAS) * K7_ROWS;
+  l.suffix_rows = l.small_rows + (n_groups == 0 ? 0 : (n_groups * kv_heads + K7_MAX_WORKERS) * K7_SMALL_ROWS);
+  l.rows = l.suffix_rows + (n_seq * kv_heads + (ratio > K7_SMALL_ROWS ? K7_MAX_CTAS : K7_MAX_WORKERS)) * ratio;
   l.plan = 0;
-  l.prefix_o = k7_up(static_cast<size_t>(16 + 32 * n_seq));
-  l.prefix_ml = l.prefix_o + k7_up(static_cast<size_t>(prefix_slots * K7_ROWS * dim * 4));
-  l.suffix_o = l.prefix_ml + k7_up(static_cast<size_t>(prefix_slots * K7_ROWS * 8));
-  l.suffix_ml = l.suffix_o + k7_up(static_cast<size_t>(suffix_slots * ratio * dim * 4));
-  l.total = l.suffix_ml + k7_up(static_cast<size_t>(suffix_slots * ratio * 8));
+  l.part_o = k7_up(static_cast<size_t>(16 * n_seq * heads));
+  l.part_ml = l.part_o + k7_up(static_cast<size_t>(l.rows * dim * 4));
+  l.total = l.part_ml + k7_up(static_cast<size_t>(l.rows * 8));
   return l;
 }
 
@@ -1105,19 +1265,25 @@ static int32_t k7_launch(const K7Params& p, cudaStream_t stream) {
   static_assert(S::PLAN + S::plan_bytes(K7_MAX_GROUPS, K7_MAX_SEQ) + 1024 <= 232448, "shared memory");
   int32_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), most);
   if (st != TOME_OK) return st;
-  kernel<<<p.ctas, K7_THREADS, bytes, stream>>>(p);
-  st = check_cuda(cudaGetLastError(), "prefix attention launch");
-  if (st != TOME_OK) return st;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(static_cast<unsigned>((static_cast<int64_t>(p.n_seq) * p.heads + 3) / 4));
-  cfg.blockDim = dim3(128);
-  cfg.stream = stream;
-  cudaLaunchAttribute attr;
+  cudaLaunchAttribute attr;  // each kernel is set up while the one before it drains
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(static_cast<unsigned>(p.ctas));
+  cfg.blockDim = dim3(K7_THREADS);
+  cfg.dynamicSmemBytes = static_cast<size_t>(bytes);
+  cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  void (*join)(K7Params) = k7_join_kernel<T, D>;
+  st = check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "prefix attention launch");
+  if (st != TOME_OK) return st;
+  // Few rows have many pieces each: a block of warps per row then, else a warp.
+  const int64_t rows = static_cast<int64_t>(p.n_seq) * p.heads;
+  const bool few = rows <= K7_MAX_CTAS * 8;
+  cfg.gridDim = dim3(static_cast<unsigned>(few ? rows : (rows + K7_JOIN_WARPS - 1) / K7_JOIN_WARPS));
+  cfg.blockDim = dim3(K7_JOIN_WARPS * 32);
+  cfg.dynamicSmemBytes = 0;
+  void (*join)(K7Params) = few ? k7_join_kernel<T, D, K7_JOIN_WARPS> : k7_join_kernel<T, D, 1>;
   return check_cuda(cudaLaunchKernelEx(&cfg, join, p), "prefix attention join launch");
 }
 
@@ -1160,12 +1326,13 @@ extern "C" int32_t tome_shared_prefix_attention(
   const K7Layout l = k7_layout(n_seq, n_groups, heads, kv_heads, head_dim);
   if (workspace == nullptr || workspace_bytes < l.total)
     return fail(TOME_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes, l.total);
-  // the cost of all items is counted in 32 bits
+  // places and rows of the workspace are counted in 32 bits
   const int64_t ratio = heads / kv_heads;
   const int64_t prefix_keys = static_cast<int64_t>(prefix_blocks) * block_size;
   const int64_t seq_keys = static_cast<int64_t>(max_blocks) * block_size;
   const int64_t row_blocks = n_groups == 0 ? 0 : n_groups + n_seq * ratio / K7_ROWS;
-  auto most = [&](int64_t keys) { return K7_ITEM_COST + K7_BIG_COST * ((keys + K7_KEYS - 1) / K7_KEYS); };
+  auto most = [&](int64_t keys) { return K7_SMALL_ITEM_COST + (keys + K7_SMALL_KEYS - 1) / K7_SMALL_KEYS; };
+  if (l.rows > 0x7fffffff) return fail(TOME_ERR_TOO_LARGE, "too many rows for one call");
   if (prefix_keys > 0x3fffffff || seq_keys > 0x3fffffff ||
       row_blocks * kv_heads * most(prefix_keys) + n_seq * kv_heads * most(seq_keys) > 0x3fffffff)
     return fail(TOME_ERR_TOO_LARGE, "the tables name too many keys for one call");
@@ -1201,12 +1368,13 @@ extern "C" int32_t tome_shared_prefix_attention(
   p.div_magic = static_cast<uint32_t>((1ull << (31 + s)) / static_cast<uint64_t>(block_size) + 1);
   p.c = scale * LOG2E;
   p.ctas = std::max(1, std::min(info.sm_count, K7_MAX_CTAS));
+  p.inv_ctas = 1.0 / p.ctas;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
-  p.plan = reinterpret_cast<int32_t*>(ws + l.plan);
-  p.prefix_o = reinterpret_cast<float*>(ws + l.prefix_o);
-  p.prefix_ml = reinterpret_cast<float2*>(ws + l.prefix_ml);
-  p.suffix_o = reinterpret_cast<float*>(ws + l.suffix_o);
-  p.suffix_ml = reinterpret_cast<float2*>(ws + l.suffix_ml);
+  p.plan = reinterpret_cast<int4*>(ws + l.plan);
+  p.part_o = reinterpret_cast<float*>(ws + l.part_o);
+  p.part_ml = reinterpret_cast<float2*>(ws + l.part_ml);
+  p.small_rows = l.small_rows;
+  p.suffix_rows = l.suffix_rows;
   p.out = out;
   p.out_lse = out_lse;
   p.status = dev_status;
