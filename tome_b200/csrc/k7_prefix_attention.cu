@@ -289,7 +289,7 @@ __device__ __forceinline__ void k7_cut_piece(K7Piece& x, int32_t at, int32_t las
 
 // The part of the item at the place `at` that lies before `last`.
 template <bool BIG>
-__device__ __noinline__ K7Piece k7_piece(const K7Params& p, const K7Plan& pl, int32_t at, int32_t last) {
+__device__ __forceinline__ K7Piece k7_piece(const K7Params& p, const K7Plan& pl, int32_t at, int32_t last) {
   K7Piece x;
   const int32_t* cum = pl.prefix[BIG];
   const int32_t in_prefix = cum[p.n_groups];
@@ -543,12 +543,11 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
   constexpr int AT_ONCE = 32 / PIECES;              // rows copied per step
   constexpr int STEPS = K7_SMALL_KEYS / AT_ONCE;
   constexpr int BLOCK = K7_SMALL_KEYS * 128;        // bytes of a 64-column block of a tile
-  // the copying side, two tiles ahead of the products
+  // the copying side, a tile ahead of the products
   K7Piece cp = {};
   int32_t cp_at = first, cp_j = 0;
   K7Pages pages = {};
-  bool cp_there = k7_next<false>(p, pl, cp, false, cp_at, last);
-  if (cp_there) pages = k7_open_pages(p, cp, cp.tile * K7_SMALL_KEYS, lane);
+  bool cp_there = true, cp_have = false;
   const int c = lane % PIECES, sub = lane / PIECES;
   const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
   const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
@@ -563,6 +562,16 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
   }
   uint32_t fill_at = 0;  // offset of the ring's stage that is filled next
   auto fill = [&]() {    // the next tile into the ring (or nothing); always one group of copies
+    if (cp_j == cp.n && cp_there) {
+      const int32_t* table = cp.table;
+      cp_there = k7_next<false>(p, pl, cp, cp_have, cp_at, last);
+      cp_have = true;
+      cp_j = 0;
+      if (cp_there) {  // the next KV head's keys lie in the same pages
+        const int32_t key0 = cp.tile * K7_SMALL_KEYS, ahead = k7_block(p, key0) - pages.first;
+        if (cp.table != table || ahead < 0 || ahead >= 32) pages = k7_open_pages(p, cp, key0, lane);
+      }
+    }
     if (cp_there) {
       const int32_t key0 = (cp.tile + cp_j) * K7_SMALL_KEYS;
       bool done = false;
@@ -596,11 +605,7 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
         }
       }
       fill_at = S::SMALL_STAGE - fill_at;
-      if (++cp_j == cp.n) {
-        cp_there = k7_next<false>(p, pl, cp, true, cp_at, last);
-        cp_j = 0;
-        if (cp_there) pages = k7_open_pages(p, cp, cp.tile * K7_SMALL_KEYS, lane);
-      }
+      ++cp_j;
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
   };
@@ -616,22 +621,23 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
     k_spot[k] = ring + k_row * 128 + (((2 * k + k_c) ^ (k_row & 7)) << 4);
     v_spot[k] = ring + S::SMALL_KV + v_row * 128 + (((2 * k + v_c) ^ (v_row & 7)) << 4);
   }
-  K7Piece x = {};
-  int32_t at = first;
   uint32_t read_at = 0;
-  for (bool have = false; k7_next<false>(p, pl, x, have, at, last); have = true) {
+  while (cp_there) {
+    // the piece of the tile that was copied last; its other tiles follow
+    const int32_t len = cp.len, tile = cp.tile, n = cp.n, rows = cp.rows;
+    const int64_t out_row = k7_out_row(p, cp.prefix, false, cp.item, worker);
     // queries, straight into the products' layout
     uint32_t qf[D / 16][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       const int32_t row = g + 8 * r, s = row / p.ratio;
       const uint32_t* src = reinterpret_cast<const uint32_t*>(
-          reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
-          static_cast<int64_t>(x.kv_head * p.ratio + (row - s * p.ratio)) * D) + (lane & 3);
+          reinterpret_cast<const T*>(p.q) + (cp.seq0 + s) * p.q_stride +
+          static_cast<int64_t>(cp.kv_head * p.ratio + (row - s * p.ratio)) * D) + (lane & 3);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) {
-        qf[k][r] = row < x.rows ? __ldg(src + 8 * k) : 0u;
-        qf[k][2 + r] = row < x.rows ? __ldg(src + 8 * k + 4) : 0u;
+        qf[k][r] = row < rows ? __ldg(src + 8 * k) : 0u;
+        qf[k][2 + r] = row < rows ? __ldg(src + 8 * k + 4) : 0u;
       }
     }
     float o[D / 8][4];
@@ -641,7 +647,7 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
       for (int e = 0; e < 4; ++e) o[k][e] = 0.0f;
     float ref[2] = {-INFINITY, -INFINITY}, sum[2] = {0.0f, 0.0f};
 #pragma unroll 1
-    for (int32_t j = 0; j < x.n; ++j) {
+    for (int32_t j = 0; j < n; ++j) {
       __syncwarp();  // the tile before, whose place is filled now, is done with
       fill();
       asm volatile("cp.async.wait_group 1;" ::: "memory");
@@ -665,7 +671,7 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
       for (int n = 0; n < 2; ++n)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[n][e] += s2[n][e];
-      const int32_t valid = x.len - (x.tile + j) * K7_SMALL_KEYS;
+      const int32_t valid = len - (tile + j) * K7_SMALL_KEYS;
       if (valid < K7_SMALL_KEYS) {
 #pragma unroll
         for (int n = 0; n < 2; ++n)
@@ -715,12 +721,11 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
         k7_mma(o[2 * k + 1], pf, f[k][2], f[k][3], T());
       }
     }
-    const int64_t out_row = k7_out_row(p, x.prefix, false, x.item, worker);
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 1);
       sum[r] += __shfl_xor_sync(0xffffffffu, sum[r], 2);
-      if (g + 8 * r < x.rows) {
+      if (g + 8 * r < rows) {
         float* dst = p.part_o + (out_row + g + 8 * r) * D + 2 * (lane & 3);
 #pragma unroll
         for (int k = 0; k < D / 8; ++k) *reinterpret_cast<float2*>(dst + 8 * k) = make_float2(o[k][2 * r], o[k][2 * r + 1]);
