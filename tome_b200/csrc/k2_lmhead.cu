@@ -31,6 +31,7 @@
 #include "combine.h"
 #include "host_common.h"
 #include "ptx.cuh"
+#include "tensor_map.h"
 
 namespace tome {
 
@@ -441,8 +442,7 @@ static int32_t get_encoder(EncodeTiledFn* out) {
   return TOME_OK;
 }
 
-// Row-major bf16 matrix [n_rows, k] with k contiguous; box = 64 columns x box_rows rows.
-static int32_t make_tmap(CUtensorMap* map, const void* ptr, int64_t n_rows, int64_t k,
+int32_t tensor_map_16bit(CUtensorMap* map, const void* ptr, int64_t n_rows, int64_t k,
                          int box_rows) {
   EncodeTiledFn enc;
   int32_t st = get_encoder(&enc);
@@ -618,9 +618,9 @@ static int32_t k2_launch(const void* hidden, const void* weight, int64_t rows, i
   const K2Plan pl = k2_plan(rows, k, vocab_local, pair ? 256 : 128);
   *plan_out = pl;
   CUtensorMap ta, tb;
-  st = make_tmap(&ta, hidden, rows, k, K2_BM);
+  st = tensor_map_16bit(&ta, hidden, rows, k, K2_BM);
   if (st != TOME_OK) return st;
-  st = make_tmap(&tb, weight, vocab_local, k, pair ? K2Cfg<true>::B_ROWS : K2Cfg<false>::B_ROWS);
+  st = tensor_map_16bit(&tb, weight, vocab_local, k, pair ? K2Cfg<true>::B_ROWS : K2Cfg<false>::B_ROWS);
   if (st != TOME_OK) return st;
   K2Params p = {};
   p.rows = rows;

@@ -27,6 +27,7 @@
 
 #include "host_common.h"
 #include "ptx.cuh"
+#include "tensor_map.h"
 
 namespace tome {
 
@@ -34,13 +35,13 @@ constexpr int K7_ROWS = 128;         // query rows of a big item at most (TMEM l
 constexpr int K7_SMALL_ROWS = 16;    // of a small one
 constexpr int K7_KEYS = 64;          // keys of a big tile
 constexpr int K7_SMALL_KEYS = 16;    // of a small one
-constexpr int K7_STAGES = 4;         // ring of big tiles
+constexpr int K7_STAGES = 4;         // of the rings of big tiles, one for keys, one for values
 constexpr int K7_SMALL_STAGES = 2;   // each warp's ring of small tiles
 constexpr int K7_TEAM_WARPS = 4;     // a team takes every other big tile
 constexpr int K7_SOFTMAX_WARPS = 2 * K7_TEAM_WARPS;
 constexpr int K7_QK_WARP = K7_SOFTMAX_WARPS;
-constexpr int K7_COPY_THREADS = 64;  // a warp fetches half of a big tile's keys and values
-constexpr int K7_PV_WARP = K7_QK_WARP + 1 + K7_COPY_THREADS / 32;
+constexpr int K7_COPY_WARP = K7_QK_WARP + 1;  // this one fetches keys, the next one values
+constexpr int K7_PV_WARP = K7_COPY_WARP + 2;
 constexpr int K7_WARPS = K7_PV_WARP + 1;         // all of them take small items
 constexpr int K7_THREADS = K7_WARPS * 32;
 // Cost of a small item besides its tiles, in tiles: the warp's ring runs dry where the queries come.
@@ -69,6 +70,7 @@ struct K7Params {
   uint32_t div_magic;         // key / block_size = (key * div_magic) >> div_shift
   int32_t div_shift;
   float c;                    // scale * log2(e)
+  bool whole_pages;           // pages of a multiple of 16 tokens: tiles go by tensor copies
   int32_t ctas;               // CTAs of the main kernel
   double inv_ctas;            // 1 / ctas
   // workspace: the pieces' rows, those of big prefix items (128 per piece), of small ones (16) from
@@ -373,26 +375,37 @@ __device__ __forceinline__ void k7_turn_pages(const K7Params& p, const K7Piece& 
   if (block - w.first < 64) w = K7Pages{w.first + 32, w.b, k7_entry(p, y, w.first + 64 + lane)};
   else w = K7Pages{block, k7_entry(p, y, block + lane), k7_entry(p, y, block + 32 + lane)};
 }
-// The page of `block` (the same for the whole warp).
-__device__ __forceinline__ int32_t k7_page(const K7Params& p, const K7Piece& y, K7Pages& w, int32_t block, int lane) {
-  k7_turn_pages(p, y, w, block, lane);
-  return __shfl_sync(0xffffffffu, w.a, block - w.first);
+// The page of each lane's `block`, at most 31 behind `first` (the same for the whole warp).
+__device__ __forceinline__ int32_t k7_page(const K7Params& p, const K7Piece& y, K7Pages& w, int32_t first,
+                                           int32_t block, int lane) {
+  k7_turn_pages(p, y, w, first, lane);
+  const int32_t rel = block - w.first;  // 0 .. 62
+  const int32_t a = __shfl_sync(0xffffffffu, w.a, rel & 31), b = __shfl_sync(0xffffffffu, w.b, rel & 31);
+  return rel < 32 ? a : b;
 }
 // The pool's row (blocks and heads flattened) of key (key0 + lane), or -1; key0 does not fall from
 // call to call, and no more than 32 keys from it on are asked for.
 __device__ __forceinline__ int32_t k7_pool_row(const K7Params& p, const K7Piece& y, K7Pages& w, int32_t key0, int lane) {
   if (key0 >= y.len) return -1;
   const int32_t key = key0 + lane, lo = k7_block(p, key0);
-  k7_turn_pages(p, y, w, lo, lane);
-  const int32_t blk = k7_block(p, min(key, y.len - 1)), rel = blk - w.first;  // 0 .. 62
-  const int32_t pa = __shfl_sync(0xffffffffu, w.a, rel & 31), pb = __shfl_sync(0xffffffffu, w.b, rel & 31);
-  const int32_t page = rel < 32 ? pa : pb;
+  const int32_t blk = k7_block(p, min(key, y.len - 1)), page = k7_page(p, y, w, lo, blk, lane);
   if (key >= y.len) return -1;
   if (page < 0 || page >= p.num_blocks) {
     k7_raise(p.status, TOME_DEV_BLOCK_OUT_OF_RANGE);  // reads as zeros, as gather does
     return -1;
   }
   return (page * p.kv_heads + y.kv_head) * p.block_size + (key - blk * p.block_size);
+}
+
+// The pool's row of key0 where it and the fifteen behind it lie in one page of whole tiles, else -1.
+// The same for the whole warp.
+__device__ __forceinline__ int32_t k7_whole_row(const K7Params& p, const K7Piece& y, K7Pages& w, int32_t key0, int lane) {
+  if (!p.whole_pages || key0 + 16 > y.len) return -1;
+  const int32_t blk = k7_block(p, key0);
+  k7_turn_pages(p, y, w, blk, lane);
+  const int32_t page = __shfl_sync(0xffffffffu, w.a, blk - w.first);
+  if (page < 0 || page >= p.num_blocks) return -1;
+  return (page * p.kv_heads + y.kv_head) * p.block_size + (key0 - blk * p.block_size);
 }
 
 // What the softmax warps need of a big piece, written by the first copying thread ahead of them;
@@ -412,19 +425,21 @@ struct K7Smem {
   static constexpr int TMEM_COLS = 512;
   static constexpr int Q_BYTES = K7_ROWS * D * 2;
   static constexpr int KV_BYTES = K7_KEYS * D * 2;
-  static constexpr int STAGE = 2 * KV_BYTES;
   static constexpr int Q = 0;                              // 2 buffers (piece parity)
-  static constexpr int KV = Q + 2 * Q_BYTES;
+  static constexpr int K = Q + 2 * Q_BYTES;                // STAGES
+  static constexpr int V = K + K7_STAGES * KV_BYTES;       // STAGES
   // small items: each warp's ring of tiles lies in the same space
   static constexpr int SMALL_KV = K7_SMALL_KEYS * D * 2;
   static constexpr int SMALL_STAGE = 2 * SMALL_KV;
   static constexpr int SMALL = K7_WARPS * K7_SMALL_STAGES * SMALL_STAGE;
-  static constexpr int MEET_ML = KV + K7_STAGES * STAGE;   // [2 teams][128] float2
+  static constexpr int MEET_ML = V + K7_STAGES * KV_BYTES; // [2 teams][128] float2
   static_assert(SMALL <= MEET_ML, "small tiles");
   static constexpr int BARS = MEET_ML + 2 * K7_ROWS * 8;
-  static constexpr int FULL = BARS;                        // STAGES
-  static constexpr int EMPTY = FULL + K7_STAGES * 8;       // STAGES
-  static constexpr int S_FULL = EMPTY + K7_STAGES * 8;     // 2 (teams), as the next two
+  static constexpr int K_FULL = BARS;                      // STAGES, as the next three
+  static constexpr int K_EMPTY = K_FULL + K7_STAGES * 8;
+  static constexpr int V_FULL = K_EMPTY + K7_STAGES * 8;
+  static constexpr int V_EMPTY = V_FULL + K7_STAGES * 8;
+  static constexpr int S_FULL = V_EMPTY + K7_STAGES * 8;   // 2 (teams), as the next two
   static constexpr int P_FULL = S_FULL + 16;
   static constexpr int O_FULL = P_FULL + 16;
   static constexpr int Q_EMPTY = O_FULL + 16;              // 2
@@ -432,7 +447,8 @@ struct K7Smem {
   static constexpr int TMEM = MEET + 16;
   static constexpr int CARD_FULL = TMEM + 16;              // K7_CARDS
   static constexpr int CARDS = CARD_FULL + K7_CARDS * 8;
-  static constexpr int PLAN = CARDS + K7_CARDS * static_cast<int>(sizeof(K7Card));
+  static constexpr int SMALL_FULL = CARDS + K7_CARDS * static_cast<int>(sizeof(K7Card));  // each warp's, STAGES
+  static constexpr int PLAN = SMALL_FULL + K7_WARPS * K7_SMALL_STAGES * 8;
   static constexpr int plan_bytes(int n_groups, int n_seq) {
     return 4 * (4 * (n_groups + 1) + n_seq + 1);
   }
@@ -530,13 +546,14 @@ __device__ __forceinline__ void k7_meet(const K7Params& p, uint32_t bar, uint32_
 }
 
 // ------------------------------------------------------------------ small items
-// A warp's run of small tiles.  It copies its own keys and values, a tile ahead, and keeps running
+// A warp's run of small tiles.  It fetches its own keys and values, a tile ahead, and keeps running
 // maximum, sum and the sums of p v in registers: nothing is shared with another warp, and twelve of
-// them hide one another's latencies.  What counts is the number of instructions per tile, since a
-// warp issues about one in eight clocks: addresses are formed once, and a tile that lies within a
-// page (pages of a multiple of 16 tokens) is copied from one address on.
+// them hide one another's latencies.  A tile that lies within a page (pages of a multiple of 16
+// tokens) comes by tensor copies, swizzled as the matrix loads want it, which one lane issues; the
+// asynchronous copies of 16 bytes that the others take keep a warp busy for 900 clocks per tile.
 template <typename T, int D>
-__device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl, uint32_t ring, int32_t worker,
+__device__ __forceinline__ void k7_small_run(const K7Params& p, const CUtensorMap* k_map, const CUtensorMap* v_map,
+                                             const K7Plan& pl, uint32_t ring, uint32_t full, int32_t worker,
                                              int32_t first, int32_t last, int lane) {
   using S = K7Smem<D>;
   constexpr int PIECES = D / 8;                     // 16-byte pieces of a row
@@ -551,17 +568,9 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
   const int c = lane % PIECES, sub = lane / PIECES;
   const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
   const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
-  const bool whole_pages = p.block_size % K7_SMALL_KEYS == 0;
-  // places in a tile of the rows r = i * AT_ONCE + sub, which repeat every eight rows
-  constexpr int TURN = 8 / AT_ONCE;
-  uint32_t spot[TURN];
-#pragma unroll
-  for (int i = 0; i < TURN; ++i) {
-    const int r = i * AT_ONCE + sub;
-    spot[i] = ring + (c >> 3) * BLOCK + r * 128 + (((c & 7) ^ r) << 4);
-  }
-  uint32_t fill_at = 0;  // offset of the ring's stage that is filled next
-  auto fill = [&]() {    // the next tile into the ring (or nothing); always one group of copies
+  uint32_t filled = 0, used = 0;  // tiles
+  uint32_t by_hand = 0;           // stages whose last tile did not come by tensor copies
+  auto fill = [&]() {  // the next tile into the ring (or nothing)
     if (cp_j == cp.n && cp_there) {
       const int32_t* table = cp.table;
       cp_there = k7_next<false>(p, pl, cp, cp_have, cp_at, last);
@@ -574,40 +583,41 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
     }
     if (cp_there) {
       const int32_t key0 = (cp.tile + cp_j) * K7_SMALL_KEYS;
-      bool done = false;
-      if (whole_pages && key0 + K7_SMALL_KEYS <= cp.len) {
-        const int32_t blk = k7_block(p, key0);
-        const int32_t page = k7_page(p, cp, pages, blk, lane);
-        if (page >= 0 && page < p.num_blocks) {
-          const int64_t off = (static_cast<int64_t>(page * p.kv_heads + cp.kv_head) * p.block_size +
-                               (key0 - blk * p.block_size) + sub) * D;
-          const T* kp = k_pool + off;
-          const T* vp = v_pool + off;
-#pragma unroll
-          for (int i = 0; i < STEPS; ++i) {
-            const uint32_t to = spot[i % TURN] + fill_at + (i / TURN) * 1024;
-            k7_copy16(to, kp + i * AT_ONCE * D, true);
-            k7_copy16(to + S::SMALL_KV, vp + i * AT_ONCE * D, true);
-          }
-          done = true;
+      const uint32_t stage = filled % K7_SMALL_STAGES, bar = full + stage * 8, dst = ring + stage * S::SMALL_STAGE;
+      const int32_t row0 = k7_whole_row(p, cp, pages, key0, lane);
+      if (row0 >= 0) {
+        if (by_hand >> stage & 1u) {  // ordinary writes before the tensor copy's
+          fence_proxy_async();
+          __syncwarp();
+          by_hand &= ~(1u << stage);
         }
-      }
-      if (!done) {
+        if (lane == 0) {
+          mbar_arrive_expect_tx(bar, S::SMALL_STAGE);
+#pragma unroll
+          for (int h = 0; h < D / 64; ++h) {
+            tma_load_2d(dst + h * BLOCK, k_map, h * 64, row0, bar);
+            tma_load_2d(dst + S::SMALL_KV + h * BLOCK, v_map, h * 64, row0, bar);
+          }
+        } else {
+          mbar_arrive(bar);
+        }
+      } else {
+        by_hand |= 1u << stage;
         const int32_t row = k7_pool_row(p, cp, pages, key0, lane);
 #pragma unroll 1
         for (int i = 0; i < STEPS; ++i) {
           const int r = i * AT_ONCE + sub;
           const int32_t from = __shfl_sync(0xffffffffu, row, r);
           const int64_t off = static_cast<int64_t>(max(from, 0)) * D;
-          const uint32_t to = ring + fill_at + (c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4);
+          const uint32_t to = dst + (c >> 3) * BLOCK + r * 128 + (((c & 7) ^ (r & 7)) << 4);
           k7_copy16(to, k_pool + off, from >= 0);
           k7_copy16(to + S::SMALL_KV, v_pool + off, from >= 0);
         }
+        k7_copies_arrive(bar);
       }
-      fill_at = S::SMALL_STAGE - fill_at;
+      ++filled;
       ++cp_j;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
   fill();
 
@@ -621,7 +631,6 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
     k_spot[k] = ring + k_row * 128 + (((2 * k + k_c) ^ (k_row & 7)) << 4);
     v_spot[k] = ring + S::SMALL_KV + v_row * 128 + (((2 * k + v_c) ^ (v_row & 7)) << 4);
   }
-  uint32_t read_at = 0;
   while (cp_there) {
     // the piece of the tile that was copied last; its other tiles follow
     const int32_t len = cp.len, tile = cp.tile, n = cp.n, rows = cp.rows;
@@ -650,8 +659,14 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
     for (int32_t j = 0; j < n; ++j) {
       __syncwarp();  // the tile before, whose place is filled now, is done with
       fill();
-      asm volatile("cp.async.wait_group 1;" ::: "memory");
-      __syncwarp();  // every lane's copies of this tile have landed
+      const uint32_t read_at = (used % K7_SMALL_STAGES) * S::SMALL_STAGE;
+      if (!mbar_wait(full + (used % K7_SMALL_STAGES) * 8, (used / K7_SMALL_STAGES) & 1u)) {
+        k7_raise(p.status, TOME_DEV_TIMEOUT);
+        asm volatile("cp.async.wait_all;" ::: "memory");
+        return;
+      }
+      __syncwarp();
+      ++used;
       float s[2][4] = {}, s2[2][4] = {};  // two chains of products for each eight keys
       uint32_t f[D / 16][4];
       // all loads of the keys first: no load's latency stands before a product
@@ -666,7 +681,6 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const K7Plan& pl
       }
 #pragma unroll
       for (int k = 0; k < D / 16; ++k) k7_ldmatrix_trans(v_spot[k % 4] + read_at + (k / 4) * BLOCK, f[k]);
-      read_at = S::SMALL_STAGE - read_at;
 #pragma unroll
       for (int n = 0; n < 2; ++n)
 #pragma unroll
@@ -875,13 +889,15 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
 }
 
 // Pipeline of the big items: two warps copy keys and values (16-byte asynchronous copies: pages of
-// any size, rows past the end filled with zeros) into a ring of four stages; one thread issues
+// any size, rows past the end filled with zeros) into rings of four stages, which drain at their own
+// pace; one thread issues
 // S = Q K^T (128 x 64 x D) and another O = P V (128 x D x 64), with P read from tensor memory and O
 // added up there (a single thread's issue, 60 clocks per product, bound the kernel: 1700 clocks
 // per tile); two teams of four softmax warps take the tiles in turn, a row per thread, each with
 // its own running maximum, sum and O, which meet at the end of a piece.
 template <typename T, int D>
-__global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Params p) {
+__global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
+    const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const K7Params p) {
   using S = K7Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -898,8 +914,10 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
 
   if (threadIdx.x == K7_QK_WARP * 32) {
     for (int i = 0; i < K7_STAGES; ++i) {
-      mbar_init(base + S::FULL + i * 8, K7_COPY_THREADS);
-      mbar_init(base + S::EMPTY + i * 8, 1);
+      mbar_init(base + S::K_FULL + i * 8, 32);
+      mbar_init(base + S::K_EMPTY + i * 8, 1);
+      mbar_init(base + S::V_FULL + i * 8, 32);
+      mbar_init(base + S::V_EMPTY + i * 8, 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(base + S::S_FULL + i * 8, 1);
@@ -909,6 +927,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
     }
     mbar_init(base + S::MEET, K7_SOFTMAX_WARPS);
     for (int i = 0; i < K7_CARDS; ++i) mbar_init(base + S::CARD_FULL + i * 8, 1);
+    for (int i = 0; i < K7_WARPS * K7_SMALL_STAGES; ++i) mbar_init(base + S::SMALL_FULL + i * 8, 32);
     fence_mbar_init();
   }
   griddep_wait();  // what the kernels before write is read from here on
@@ -946,7 +965,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
     } else if (warp == K7_QK_WARP) {
       // ---------------------------------------------------------- tensor-core products
       if (lane == 0) {
-        const uint64_t q_desc = k7_desc_k(base + S::Q), k_desc = k7_desc_k(base + S::KV);
+        const uint64_t q_desc = k7_desc_k(base + S::Q), k_desc = k7_desc_k(base + S::K);
         uint32_t u = 0, piece = 0;
         bool ok = true;
         K7Piece x;
@@ -955,7 +974,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           for (int32_t j = 0; j < x.n; ++j, ++u) {
             const uint32_t stage = u % K7_STAGES, team = u & 1u;
             // keys (and queries) are there, and the team has read the scores that lie where these go
-            if (!mbar_wait(base + S::FULL + stage * 8, (u / K7_STAGES) & 1u) ||
+            if (!mbar_wait(base + S::K_FULL + stage * 8, (u / K7_STAGES) & 1u) ||
                 (u >= 2 && !mbar_wait(base + S::P_FULL + team * 8, ((u >> 1) - 1) & 1u))) {
               k7_raise(p.status, TOME_DEV_TIMEOUT);
               ok = false;
@@ -963,12 +982,13 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
             }
             fence_proxy_async();  // the copies are ordinary writes: visible to the tensor core from here
             tc_fence_after_sync();
-            const uint64_t a = q_desc + (piece & 1u) * (S::Q_BYTES >> 4), b = k_desc + stage * (S::STAGE >> 4);
+            const uint64_t a = q_desc + (piece & 1u) * (S::Q_BYTES >> 4), b = k_desc + stage * (S::KV_BYTES >> 4);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
               umma_bf16_ss(tmem + team * K7_KEYS, a + (k / 4) * (K7_ROWS * 128 >> 4) + 2 * (k % 4),
                            b + (k / 4) * (K7_KEYS * 128 >> 4) + 2 * (k % 4), k7_idesc<T>(K7_KEYS, false), k != 0);
             umma_commit(base + S::S_FULL + team * 8);
+            umma_commit(base + S::K_EMPTY + stage * 8);
             if (j == x.n - 1) umma_commit(base + S::Q_EMPTY + (piece & 1u) * 8);
           }
         }
@@ -976,7 +996,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
       __syncwarp();
     } else if (warp == K7_PV_WARP) {
       if (lane == 0) {
-        const uint64_t v_desc = k7_desc_mn(base + S::KV + S::KV_BYTES, K7_KEYS * 128);
+        const uint64_t v_desc = k7_desc_mn(base + S::V, K7_KEYS * 128);
         uint32_t u = 0, piece = 0;
         bool ok = true;
         K7Piece x;
@@ -985,19 +1005,19 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           for (int32_t j = 0; j < x.n; ++j, ++u) {
             const uint32_t stage = u % K7_STAGES, team = u & 1u;
             if (!mbar_wait(base + S::P_FULL + team * 8, (u >> 1) & 1u) ||
-                !mbar_wait(base + S::FULL + stage * 8, (u / K7_STAGES) & 1u)) {  // (done long ago)
+                !mbar_wait(base + S::V_FULL + stage * 8, (u / K7_STAGES) & 1u)) {
               k7_raise(p.status, TOME_DEV_TIMEOUT);
               ok = false;
               break;
             }
             fence_proxy_async();
             tc_fence_after_sync();
-            const uint64_t b = v_desc + stage * (S::STAGE >> 4);
+            const uint64_t b = v_desc + stage * (S::KV_BYTES >> 4);
             const uint32_t d = tmem + S::O_COL + team * D, a = tmem + S::P_COL + team * (K7_KEYS / 2);
 #pragma unroll
             for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 8 columns of P, 16 rows of V
               umma_f16_ts(d, a + 8 * k, b + (2048 >> 4) * k, k7_idesc<T>(D, true), j > 1 || k != 0);
-            umma_commit(base + S::EMPTY + stage * 8);
+            umma_commit(base + S::V_EMPTY + stage * 8);
             umma_commit(base + S::O_FULL + team * 8);
           }
         }
@@ -1012,35 +1032,35 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
     } else if (warp < K7_PV_WARP) {
       // ---------------------------------------------------------- copies
       constexpr int PIECES = D / 8;                  // 16-byte pieces of a row
-      constexpr int AT_ONCE = 32 / PIECES;           // rows that a warp copies per step
-      constexpr int STEPS = 32 / AT_ONCE;            // a warp has 32 of the 64 keys
-      const int cw = warp - (K7_QK_WARP + 1);
+      constexpr int AT_ONCE = 32 / PIECES;           // rows copied per step
+      constexpr int STEPS = 16 / AT_ONCE;            // for sixteen rows
+      const bool keys = warp == K7_COPY_WARP;        // the other one: values
       const int c = lane % PIECES, sub = lane / PIECES;
-      const int my_row = cw * 32;
-      const T* k_pool = reinterpret_cast<const T*>(p.k_pool) + c * 8;
-      const T* v_pool = reinterpret_cast<const T*>(p.v_pool) + c * 8;
-      const uint32_t area = base + S::KV + (c >> 3) * (K7_KEYS * 128);
+      const T* pool = reinterpret_cast<const T*>(keys ? p.k_pool : p.v_pool) + c * 8;
+      const CUtensorMap* map = keys ? &k_map : &v_map;
+      const uint32_t area = base + (keys ? S::K : S::V);
+      const uint32_t full = base + (keys ? S::K_FULL : S::V_FULL), empty = base + (keys ? S::K_EMPTY : S::V_EMPTY);
       auto show = [&](const K7Piece& y, uint32_t index, bool there) {  // to the softmax warps
-        if (cw == 0 && lane == 0) {
+        if (keys && lane == 0) {
           cards[index % K7_CARDS] = K7Card{y.len, y.tile, there ? y.n : 0, y.rows, y.item, y.prefix ? 1 : 0};
           mbar_arrive(base + S::CARD_FULL + (index % K7_CARDS) * 8);
         }
       };
-      uint32_t t = 0, piece = 0;
+      uint32_t t = 0, piece = 0, by_hand = 0;
       bool ok = true;
       int32_t at = first;
       K7Piece x = {};
       K7Pages pages = {};
       bool there = k7_next<true>(p, pl, x, false, at, last);
       show(x, 0, there);
-      if (there) pages = k7_open_pages(p, x, x.tile * K7_KEYS + my_row, lane);
+      if (there) pages = k7_open_pages(p, x, x.tile * K7_KEYS, lane);
       while (there && ok) {
-        if (piece >= 2 && !mbar_wait(base + S::Q_EMPTY + (piece & 1u) * 8, ((piece >> 1) - 1) & 1u)) {
+        if (keys && piece >= 2 && !mbar_wait(base + S::Q_EMPTY + (piece & 1u) * 8, ((piece >> 1) - 1) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
           ok = false;
           break;
         }
-        for (int i = cw * AT_ONCE + sub; i < x.rows; i += 2 * AT_ONCE) {
+        for (int i = sub; keys && i < x.rows; i += AT_ONCE) {  // the queries come with the first keys
           const int32_t row = x.row0 + i, s = row / p.ratio;
           const T* src = reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
                          static_cast<int64_t>(x.kv_head * p.ratio + (row - s * p.ratio)) * D + c * 8;
@@ -1056,26 +1076,59 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
           if (j + 1 == x.n) {  // the piece behind is looked up while this one's loads are under way
             next_there = k7_next<true>(p, pl, next, true, at, last);
             show(next, piece + 1, next_there);
-            if (next_there) next_pages = k7_open_pages(p, next, next.tile * K7_KEYS + my_row, lane);
+            if (next_there) next_pages = k7_open_pages(p, next, next.tile * K7_KEYS, lane);
           }
-          if (t >= K7_STAGES && !mbar_wait(base + S::EMPTY + stage * 8, (t / K7_STAGES - 1) & 1u)) {
+          if (t >= K7_STAGES && !mbar_wait(empty + stage * 8, (t / K7_STAGES - 1) & 1u)) {
             k7_raise(p.status, TOME_DEV_TIMEOUT);
             ok = false;
             break;
           }
           __syncwarp();
-          const int32_t pool_row = k7_pool_row(p, x, pages, (x.tile + j) * K7_KEYS + my_row, lane);
-          const uint32_t dst = area + stage * S::STAGE;
-#pragma unroll
-          for (int i = 0; i < STEPS; ++i) {
-            const int r = my_row + i * AT_ONCE + sub;
-            const int32_t from = __shfl_sync(0xffffffffu, pool_row, i * AT_ONCE + sub);
-            const int64_t off = static_cast<int64_t>(max(from, 0)) * D;
-            const uint32_t to = dst + r * 128 + (((c & 7) ^ (r & 7)) << 4);
-            k7_copy16(to, k_pool + off, from >= 0);
-            k7_copy16(to + S::KV_BYTES, v_pool + off, from >= 0);
+          const uint32_t dst = area + stage * S::KV_BYTES;
+          const int32_t key0 = (x.tile + j) * K7_KEYS;
+          // pool rows of the tile's four groups of sixteen keys, one per lane, where whole pages hold them
+          const int32_t group = key0 + 16 * (lane & 3);
+          int32_t row = -1;
+          bool whole = p.whole_pages && key0 + K7_KEYS <= x.len;
+          if (whole) {
+            const int32_t blk = k7_block(p, group), page = k7_page(p, x, pages, k7_block(p, key0), blk, lane);
+            if (page >= 0 && page < p.num_blocks)
+              row = (page * p.kv_heads + x.kv_head) * p.block_size + (group - blk * p.block_size);
+            whole = __all_sync(0xffffffffu, row >= 0);
           }
-          k7_copies_arrive(base + S::FULL + stage * 8);
+          // (a piece's queries come by asynchronous copies, which every lane's arrival waits for)
+          if (whole) {
+            if (by_hand >> stage & 1u) {  // ordinary writes before the tensor copies'
+              fence_proxy_async();
+              __syncwarp();
+              by_hand &= ~(1u << stage);
+            }
+            int32_t rows[K7_KEYS / 16];
+#pragma unroll
+            for (int h = 0; h < K7_KEYS / 16; ++h) rows[h] = __shfl_sync(0xffffffffu, row, h);
+            if (lane == 0) {
+              mbar_expect_tx(full + stage * 8, S::KV_BYTES);
+#pragma unroll
+              for (int h = 0; h < K7_KEYS / 16; ++h)
+#pragma unroll
+                for (int b = 0; b < D / 64; ++b)
+                  tma_load_2d(dst + b * (K7_KEYS * 128) + h * 2048, map, b * 64, rows[h], full + stage * 8);
+            }
+          } else {
+            by_hand |= 1u << stage;
+#pragma unroll 1
+            for (int h = 0; h < K7_KEYS; h += 16) {
+              const int32_t pool_row = k7_pool_row(p, x, pages, key0 + h, lane);
+#pragma unroll 1
+              for (int i = 0; i < STEPS; ++i) {
+                const int r = i * AT_ONCE + sub;
+                const int32_t from = __shfl_sync(0xffffffffu, pool_row, r);
+                k7_copy16(dst + (c >> 3) * (K7_KEYS * 128) + (h + r) * 128 + (((c & 7) ^ (r & 7)) << 4),
+                          pool + static_cast<int64_t>(max(from, 0)) * D, from >= 0);
+              }
+            }
+          }
+          k7_copies_arrive(full + stage * 8);
         }
         x = next;
         pages = next_pages;
@@ -1084,6 +1137,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
       }
       asm volatile("cp.async.wait_all;" ::: "memory");
     }
+    fence_proxy_async();  // the space is filled by tensor copies again
     tc_fence_before_sync();
     __syncthreads();
     if (warp == K7_QK_WARP) {
@@ -1126,7 +1180,8 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(const K7Par
   // the first workers are spread over the CTAs
   const int32_t worker = warp * gridDim.x + blockIdx.x;
   if (worker < small.workers)
-    k7_small_run<T, D>(p, pl, base + warp * (K7_SMALL_STAGES * S::SMALL_STAGE), worker, small.begin(worker),
+    k7_small_run<T, D>(p, &k_map, &v_map, pl, base + warp * (K7_SMALL_STAGES * S::SMALL_STAGE),
+                       base + S::SMALL_FULL + warp * (K7_SMALL_STAGES * 8), worker, small.begin(worker),
                        small.begin(worker + 1), lane);
 }
 
@@ -1263,13 +1318,21 @@ static int32_t k7_shape(int64_t n_seq, int64_t n_groups, int64_t heads, int64_t 
 template <typename T, int D>
 static int32_t k7_launch(const K7Params& p, cudaStream_t stream) {
   using S = K7Smem<D>;
-  void (*kernel)(K7Params) = k7_attention_kernel<T, D>;
+  void (*kernel)(CUtensorMap, CUtensorMap, K7Params) = k7_attention_kernel<T, D>;
   const int bytes = S::PLAN + S::plan_bytes(p.n_groups, p.n_seq) + 1024;
   // set once for the largest plan, so that no later call has to raise it
   const int most = S::PLAN + S::plan_bytes(K7_MAX_GROUPS, K7_MAX_SEQ) + 1024;
   static_assert(S::PLAN + S::plan_bytes(K7_MAX_GROUPS, K7_MAX_SEQ) + 1024 <= 232448, "shared memory");
   int32_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), most);
   if (st != TOME_OK) return st;
+  // the pools as matrices of 64-column blocks, sixteen rows at a time
+  CUtensorMap k_map = {}, v_map = {};
+  if (p.whole_pages) {
+    const int64_t rows = static_cast<int64_t>(p.num_blocks) * p.kv_heads * p.block_size;
+    st = tensor_map_16bit(&k_map, p.k_pool, rows, D, 16);
+    if (st == TOME_OK) st = tensor_map_16bit(&v_map, p.v_pool, rows, D, 16);
+    if (st != TOME_OK) return st;
+  }
   cudaLaunchAttribute attr;  // each kernel is set up while the one before it drains
   attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr.val.programmaticStreamSerializationAllowed = 1;
@@ -1280,7 +1343,7 @@ static int32_t k7_launch(const K7Params& p, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  st = check_cuda(cudaLaunchKernelEx(&cfg, kernel, p), "prefix attention launch");
+  st = check_cuda(cudaLaunchKernelEx(&cfg, kernel, k_map, v_map, p), "prefix attention launch");
   if (st != TOME_OK) return st;
   // Few rows have many pieces each: a block of warps per row then, else a warp.
   const int64_t rows = static_cast<int64_t>(p.n_seq) * p.heads;
@@ -1372,6 +1435,7 @@ extern "C" int32_t tome_shared_prefix_attention(
   p.div_shift = 31 + s;
   p.div_magic = static_cast<uint32_t>((1ull << (31 + s)) / static_cast<uint64_t>(block_size) + 1);
   p.c = scale * LOG2E;
+  p.whole_pages = block_size % 16 == 0 && num_blocks > 0;
   p.ctas = std::max(1, std::min(info.sm_count, K7_MAX_CTAS));
   p.inv_ctas = 1.0 / p.ctas;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
