@@ -35,20 +35,24 @@ constexpr int K7_ROWS = 128;         // query rows of a big item at most (TMEM l
 constexpr int K7_SMALL_ROWS = 16;    // of a small one
 constexpr int K7_KEYS = 64;          // keys of a big tile
 constexpr int K7_SMALL_KEYS = 16;    // of a small one
-constexpr int K7_STAGES = 4;         // of the rings of big tiles, one for keys, one for values
+// Rings of big tiles.  Even, so that a team meets a stage's phases one by one; values stay longer,
+// from their load until the softmax of their tile is done.
+constexpr int K7_K_STAGES = 4;
+constexpr int K7_V_STAGES = 6;
 constexpr int K7_SMALL_STAGES = 2;   // each warp's ring of small tiles
 constexpr int K7_TEAM_WARPS = 4;     // a team takes every other big tile
 constexpr int K7_SOFTMAX_WARPS = 2 * K7_TEAM_WARPS;
-constexpr int K7_QK_WARP = K7_SOFTMAX_WARPS;
-constexpr int K7_COPY_WARP = K7_QK_WARP + 1;  // this one fetches keys, the next one values
-constexpr int K7_PV_WARP = K7_COPY_WARP + 2;
-constexpr int K7_WARPS = K7_PV_WARP + 1;         // all of them take small items
+constexpr int K7_ISSUE_WARP = K7_SOFTMAX_WARPS;        // issues the products of the first team,
+constexpr int K7_ISSUE_WARP_2 = K7_ISSUE_WARP + 1;     // of the second one
+constexpr int K7_COPY_WARP = K7_ISSUE_WARP_2 + 1;      // fetches keys, the next one values
+constexpr int K7_WARPS = K7_COPY_WARP + 2;             // all of them take small items
 constexpr int K7_THREADS = K7_WARPS * 32;
 // Cost of a small item besides its tiles, in tiles: the warp's ring runs dry where the queries come.
 constexpr int K7_SMALL_ITEM_COST = 2;
-// Cards of pieces in flight.  One is written over four pieces later; the copying warps are at most
-// two pieces ahead of a Q buffer's release, and that comes after the softmax warps took the card.
-constexpr int K7_CARDS = 4;
+// Cards of pieces in flight.  The warp that writes them is at most the ring's tiles ahead of the
+// softmax warps (each piece has a tile), and a card is written over more pieces later than that.
+constexpr int K7_CARDS = 8;
+static_assert(K7_CARDS >= K7_K_STAGES + 3, "cards");
 constexpr int K7_MAX_SEQ = 2048;
 constexpr int K7_MAX_GROUPS = 512;
 // The split takes at most this many CTAs (one per SM); the workspace does not depend on the
@@ -67,8 +71,8 @@ struct K7Params {
   const int32_t* tables;         // [n_seq, seq_blocks]
   const int32_t* lengths;        // [n_seq]
   int32_t n_seq, n_groups, heads, kv_heads, ratio, block_size, prefix_blocks, seq_blocks, num_blocks;
-  uint32_t div_magic;         // key / block_size = (key * div_magic) >> div_shift
-  int32_t div_shift;
+  uint32_t div_magic, ratio_magic;  // x / block_size and x / ratio, see k7_div
+  int32_t div_shift, ratio_shift;
   float c;                    // scale * log2(e)
   bool whole_pages;           // pages of a multiple of 16 tokens: tiles go by tensor copies
   int32_t ctas;               // CTAs of the main kernel
@@ -89,6 +93,11 @@ struct K7Params {
 
 __device__ __forceinline__ void k7_raise(int32_t* status, int32_t bit) {
   if (status != nullptr) atomicOr(status, bit);
+}
+
+// x / d for 0 <= x < 2^31 with s = ceil(log2 d), magic = floor(2^(31+s) / d) + 1, shift = 31 + s.
+__device__ __forceinline__ int32_t k7_div(int32_t x, uint32_t magic, int32_t shift) {
+  return static_cast<int32_t>(static_cast<uint64_t>(x) * magic >> shift);
 }
 
 // Length of a table's keys: never negative, never past the table.
@@ -159,6 +168,7 @@ __device__ __forceinline__ void k7_build_plan(const K7Params& p, const K7Plan& p
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         const int i = base + 32 * k + lane;
+        if (base + 32 * k > p.n_groups) break;
         const int32_t v = max(top, k7_scan_max(min(max(f.v[k], 0), p.n_seq), lane));
         if (i <= p.n_groups) pl.group[i] = v;
         top = __shfl_sync(0xffffffffu, v, 31);
@@ -360,7 +370,7 @@ struct K7Pages {
   int32_t first, a, b;
 };
 __device__ __forceinline__ int32_t k7_block(const K7Params& p, int32_t key) {
-  return static_cast<int32_t>(static_cast<uint64_t>(key) * p.div_magic >> p.div_shift);
+  return k7_div(key, p.div_magic, p.div_shift);
 }
 __device__ __forceinline__ int32_t k7_entry(const K7Params& p, const K7Piece& y, int32_t block) {
   return block <= k7_block(p, y.len - 1) ? __ldg(y.table + block) : -1;
@@ -411,7 +421,7 @@ __device__ __forceinline__ int32_t k7_whole_row(const K7Params& p, const K7Piece
 // What the softmax warps need of a big piece, written by the first copying thread ahead of them;
 // n = 0 behind the last one.
 struct K7Card {
-  int32_t len, tile, n, rows, item, prefix;
+  int32_t len, tile, n, rows, item, prefix, seq0, row0, kv_head;
 };
 
 // ------------------------------------------------------------------ shared memory and products
@@ -425,25 +435,25 @@ struct K7Smem {
   static constexpr int TMEM_COLS = 512;
   static constexpr int Q_BYTES = K7_ROWS * D * 2;
   static constexpr int KV_BYTES = K7_KEYS * D * 2;
-  static constexpr int Q = 0;                              // 2 buffers (piece parity)
-  static constexpr int K = Q + 2 * Q_BYTES;                // STAGES
-  static constexpr int V = K + K7_STAGES * KV_BYTES;       // STAGES
+  static constexpr int Q = 0;
+  static constexpr int K = Q + Q_BYTES;                    // K_STAGES
+  static constexpr int V = K + K7_K_STAGES * KV_BYTES;     // V_STAGES
   // small items: each warp's ring of tiles lies in the same space
   static constexpr int SMALL_KV = K7_SMALL_KEYS * D * 2;
   static constexpr int SMALL_STAGE = 2 * SMALL_KV;
   static constexpr int SMALL = K7_WARPS * K7_SMALL_STAGES * SMALL_STAGE;
-  static constexpr int MEET_ML = V + K7_STAGES * KV_BYTES; // [2 teams][128] float2
+  static constexpr int MEET_ML = V + K7_V_STAGES * KV_BYTES; // [2 teams][128] float2
   static_assert(SMALL <= MEET_ML, "small tiles");
   static constexpr int BARS = MEET_ML + 2 * K7_ROWS * 8;
-  static constexpr int K_FULL = BARS;                      // STAGES, as the next three
-  static constexpr int K_EMPTY = K_FULL + K7_STAGES * 8;
-  static constexpr int V_FULL = K_EMPTY + K7_STAGES * 8;
-  static constexpr int V_EMPTY = V_FULL + K7_STAGES * 8;
-  static constexpr int S_FULL = V_EMPTY + K7_STAGES * 8;   // 2 (teams), as the next two
+  static constexpr int K_FULL = BARS;                      // stages, as the next three
+  static constexpr int K_EMPTY = K_FULL + K7_K_STAGES * 8;
+  static constexpr int V_FULL = K_EMPTY + K7_K_STAGES * 8;
+  static constexpr int V_EMPTY = V_FULL + K7_V_STAGES * 8;
+  static constexpr int S_FULL = V_EMPTY + K7_V_STAGES * 8; // 2 (teams), as the next three
   static constexpr int P_FULL = S_FULL + 16;
   static constexpr int O_FULL = P_FULL + 16;
-  static constexpr int Q_EMPTY = O_FULL + 16;              // 2
-  static constexpr int MEET = Q_EMPTY + 16;                // the softmax warps among themselves
+  static constexpr int Q_FULL = O_FULL + 16;
+  static constexpr int MEET = Q_FULL + 16;                 // the softmax warps among themselves
   static constexpr int TMEM = MEET + 16;
   static constexpr int CARD_FULL = TMEM + 16;              // K7_CARDS
   static constexpr int CARDS = CARD_FULL + K7_CARDS * 8;
@@ -639,7 +649,7 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const CUtensorMa
     uint32_t qf[D / 16][4];
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
-      const int32_t row = g + 8 * r, s = row / p.ratio;
+      const int32_t row = g + 8 * r, s = k7_div(row, p.ratio_magic, p.ratio_shift);
       const uint32_t* src = reinterpret_cast<const uint32_t*>(
           reinterpret_cast<const T*>(p.q) + (cp.seq0 + s) * p.q_stride +
           static_cast<int64_t>(cp.kv_head * p.ratio + (row - s * p.ratio)) * D) + (lane & 3);
@@ -763,6 +773,19 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
   const bool active = (warp % K7_TEAM_WARPS) * 32 < x.rows;  // warps without a row only keep step
   const uint32_t o_addr = tmem + lanes + S::O_COL;
   bool ok = true;
+  {  // the piece's queries, a warp's share of the rows (nothing reads the last piece's any more)
+    constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES;
+    const int c = lane % PIECES;
+    for (int i = warp * AT_ONCE + lane / PIECES; i < x.rows; i += K7_SOFTMAX_WARPS * AT_ONCE) {
+      const int32_t r = x.row0 + i, s = k7_div(r, p.ratio_magic, p.ratio_shift);
+      k7_copy16(base + S::Q + (c >> 3) * (K7_ROWS * 128) + i * 128 + (((c & 7) ^ (i & 7)) << 4),
+                reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
+                    static_cast<int64_t>(x.kv_head * p.ratio + (r - s * p.ratio)) * D + c * 8,
+                true);
+    }
+    for (uint32_t t = 0; t < 2; ++t)  // tell the teams that have a tile of the piece
+      if (x.n > 1 || (u & 1u) == t) k7_copies_arrive(base + S::Q_FULL + t * 8);
+  }
   // `ref` is what the exponents are relative to, in the log2 domain.  It follows the row's maximum
   // only when that has grown by more than 2^8: the sums in tensor memory then have to be
   // rescaled, which hardly ever happens after the first tiles.
@@ -888,13 +911,13 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
   return ok;
 }
 
-// Pipeline of the big items: two warps copy keys and values (16-byte asynchronous copies: pages of
-// any size, rows past the end filled with zeros) into rings of four stages, which drain at their own
-// pace; one thread issues
-// S = Q K^T (128 x 64 x D) and another O = P V (128 x D x 64), with P read from tensor memory and O
-// added up there (a single thread's issue, 60 clocks per product, bound the kernel: 1700 clocks
-// per tile); two teams of four softmax warps take the tiles in turn, a row per thread, each with
-// its own running maximum, sum and O, which meet at the end of a piece.
+// Pipeline of the big items: two warps fetch keys and values (tensor copies of 16 rows where pages
+// allow it, else asynchronous copies of 16 bytes; rows past the end are zeros) into rings of four
+// stages, which drain at their own pace.  Two teams take the tiles in turn: a thread issues
+// S = Q K^T (128 x 64 x D) and O += P V (128 x D x 64, P read from tensor memory), four warps own a row
+// per thread and keep its running maximum and sum; the teams' O meet at the end of a piece.  (A
+// thread needs about 60 clocks to issue a product: one thread for both teams bound the kernel at
+// 1700 clocks per tile.)
 template <typename T, int D>
 __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
     const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const K7Params p) {
@@ -912,10 +935,12 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
   pl.suffix = pl.prefix[1] + p.n_groups + 1;
   K7Card* const cards = reinterpret_cast<K7Card*>(smem + S::CARDS);
 
-  if (threadIdx.x == K7_QK_WARP * 32) {
-    for (int i = 0; i < K7_STAGES; ++i) {
+  if (threadIdx.x == K7_ISSUE_WARP * 32) {
+    for (int i = 0; i < K7_K_STAGES; ++i) {
       mbar_init(base + S::K_FULL + i * 8, 32);
       mbar_init(base + S::K_EMPTY + i * 8, 1);
+    }
+    for (int i = 0; i < K7_V_STAGES; ++i) {
       mbar_init(base + S::V_FULL + i * 8, 32);
       mbar_init(base + S::V_EMPTY + i * 8, 1);
     }
@@ -923,7 +948,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
       mbar_init(base + S::S_FULL + i * 8, 1);
       mbar_init(base + S::P_FULL + i * 8, K7_TEAM_WARPS);
       mbar_init(base + S::O_FULL + i * 8, 1);
-      mbar_init(base + S::Q_EMPTY + i * 8, 1);
+      mbar_init(base + S::Q_FULL + i * 8, K7_SOFTMAX_WARPS * 32);
     }
     mbar_init(base + S::MEET, K7_SOFTMAX_WARPS);
     for (int i = 0; i < K7_CARDS; ++i) mbar_init(base + S::CARD_FULL + i * 8, 1);
@@ -938,7 +963,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
   const K7Split small(k7_cost(p, pl, false), p.ctas * K7_WARPS, p.inv_ctas / K7_WARPS, false);
 
   if (big.cost > 0) {  // (the same for all threads of all CTAs)
-    if (warp == K7_QK_WARP) {
+    if (warp == K7_ISSUE_WARP) {
       tmem_alloc(base + S::TMEM, S::TMEM_COLS);
       tmem_relinquish();
     }
@@ -962,74 +987,67 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
         const int64_t out_row = k7_out_row(p, x.prefix != 0, true, x.item, blockIdx.x);
         ok = k7_big_piece<T, D>(p, smem, base, tmem, x, u, warp, lane, p.part_o + out_row * D, p.part_ml + out_row, met);
       }
-    } else if (warp == K7_QK_WARP) {
-      // ---------------------------------------------------------- tensor-core products
+    } else if (warp == K7_ISSUE_WARP || warp == K7_ISSUE_WARP_2) {
+      // ---------------------------------------------------------- tensor-core products of a team
       if (lane == 0) {
+        const uint32_t team = warp == K7_ISSUE_WARP ? 0u : 1u;
         const uint64_t q_desc = k7_desc_k(base + S::Q), k_desc = k7_desc_k(base + S::K);
-        uint32_t u = 0, piece = 0;
-        bool ok = true;
+        const uint64_t v_desc = k7_desc_mn(base + S::V, K7_KEYS * 128);
+        const uint32_t s_addr = tmem + team * K7_KEYS, o_addr = tmem + S::O_COL + team * D;
+        const uint32_t p_addr = tmem + S::P_COL + team * (K7_KEYS / 2);
+        uint32_t u = 0, piece = 0, pieces = 0, last_mine = 0;  // `pieces`: those with a tile of the team
+        bool ok = true, any = false;
+        // P of the team's tile `i` is there, and its S is read
+        auto wait_p = [&](uint32_t i) {
+          if (!mbar_wait(base + S::P_FULL + team * 8, (i >> 1) & 1u)) ok = false;
+        };
+        auto multiply_pv = [&](uint32_t i, bool add) {  // O (+)= P V of tile i
+          const uint32_t stage = i % K7_V_STAGES;
+          if (!mbar_wait(base + S::V_FULL + stage * 8, (i / K7_V_STAGES) & 1u)) ok = false;
+          fence_proxy_async();  // tiles that did not come by tensor copies are ordinary writes
+          tc_fence_after_sync();
+          const uint64_t b = v_desc + stage * (S::KV_BYTES >> 4);
+#pragma unroll
+          for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 8 columns of P, 16 rows of V
+            umma_f16_ts(o_addr, p_addr + 8 * k, b + (2048 >> 4) * k, k7_idesc<T>(D, true), add || k != 0);
+          umma_commit(base + S::O_FULL + team * 8);
+          umma_commit(base + S::V_EMPTY + stage * 8);
+        };
         K7Piece x;
         int32_t at = first;
         for (; ok && k7_next<true>(p, pl, x, piece > 0, at, last); ++piece) {
-          for (int32_t j = 0; j < x.n; ++j, ++u) {
-            const uint32_t stage = u % K7_STAGES, team = u & 1u;
-            // keys (and queries) are there, and the team has read the scores that lie where these go
-            if (!mbar_wait(base + S::K_FULL + stage * 8, (u / K7_STAGES) & 1u) ||
-                (u >= 2 && !mbar_wait(base + S::P_FULL + team * 8, ((u >> 1) - 1) & 1u))) {
-              k7_raise(p.status, TOME_DEV_TIMEOUT);
-              ok = false;
-              break;
-            }
-            fence_proxy_async();  // the copies are ordinary writes: visible to the tensor core from here
+          const uint32_t end = u + x.n, mine = u + ((u ^ team) & 1u);
+          for (uint32_t i = mine; i < end && ok; i += 2) {
+            const uint32_t stage = i % K7_K_STAGES;
+            if (i == mine && !mbar_wait(base + S::Q_FULL + team * 8, pieces++ & 1u)) ok = false;
+            if (!mbar_wait(base + S::K_FULL + stage * 8, (i / K7_K_STAGES) & 1u)) ok = false;
+            if (i > mine) wait_p(i - 2);
+            if (!ok) break;
+            fence_proxy_async();
             tc_fence_after_sync();
-            const uint64_t a = q_desc + (piece & 1u) * (S::Q_BYTES >> 4), b = k_desc + stage * (S::KV_BYTES >> 4);
+            const uint64_t a = q_desc, b = k_desc + stage * (S::KV_BYTES >> 4);
 #pragma unroll
             for (int k = 0; k < D / 16; ++k)
-              umma_bf16_ss(tmem + team * K7_KEYS, a + (k / 4) * (K7_ROWS * 128 >> 4) + 2 * (k % 4),
+              umma_bf16_ss(s_addr, a + (k / 4) * (K7_ROWS * 128 >> 4) + 2 * (k % 4),
                            b + (k / 4) * (K7_KEYS * 128 >> 4) + 2 * (k % 4), k7_idesc<T>(K7_KEYS, false), k != 0);
             umma_commit(base + S::S_FULL + team * 8);
             umma_commit(base + S::K_EMPTY + stage * 8);
-            if (j == x.n - 1) umma_commit(base + S::Q_EMPTY + (piece & 1u) * 8);
+            if (i > mine) multiply_pv(i - 2, i - 2 > mine);
+            last_mine = i;
           }
-        }
-      }
-      __syncwarp();
-    } else if (warp == K7_PV_WARP) {
-      if (lane == 0) {
-        const uint64_t v_desc = k7_desc_mn(base + S::V, K7_KEYS * 128);
-        uint32_t u = 0, piece = 0;
-        bool ok = true;
-        K7Piece x;
-        int32_t at = first;
-        for (; ok && k7_next<true>(p, pl, x, piece > 0, at, last); ++piece) {
-          for (int32_t j = 0; j < x.n; ++j, ++u) {
-            const uint32_t stage = u % K7_STAGES, team = u & 1u;
-            if (!mbar_wait(base + S::P_FULL + team * 8, (u >> 1) & 1u) ||
-                !mbar_wait(base + S::V_FULL + stage * 8, (u / K7_STAGES) & 1u)) {
-              k7_raise(p.status, TOME_DEV_TIMEOUT);
-              ok = false;
-              break;
-            }
-            fence_proxy_async();
-            tc_fence_after_sync();
-            const uint64_t b = v_desc + stage * (S::KV_BYTES >> 4);
-            const uint32_t d = tmem + S::O_COL + team * D, a = tmem + S::P_COL + team * (K7_KEYS / 2);
-#pragma unroll
-            for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 8 columns of P, 16 rows of V
-              umma_f16_ts(d, a + 8 * k, b + (2048 >> 4) * k, k7_idesc<T>(D, true), j > 1 || k != 0);
-            umma_commit(base + S::V_EMPTY + stage * 8);
-            umma_commit(base + S::O_FULL + team * 8);
+          if (mine < end && ok) {  // the softmax warps wait for the last tile's O
+            any = true;
+            wait_p(last_mine);
+            if (ok) multiply_pv(last_mine, last_mine > mine);
           }
+          u = end;
         }
         // nothing may still be under way when the space is used otherwise
-        for (uint32_t i = u > 2 ? u - 2 : 0; i < u && ok; ++i)
-          if (!mbar_wait(base + S::O_FULL + (i & 1u) * 8, (i >> 1) & 1u)) {
-            k7_raise(p.status, TOME_DEV_TIMEOUT);
-            ok = false;
-          }
+        if (ok && any && !mbar_wait(base + S::O_FULL + team * 8, (last_mine >> 1) & 1u)) ok = false;
+        if (!ok) k7_raise(p.status, TOME_DEV_TIMEOUT);
       }
       __syncwarp();
-    } else if (warp < K7_PV_WARP) {
+    } else {
       // ---------------------------------------------------------- copies
       constexpr int PIECES = D / 8;                  // 16-byte pieces of a row
       constexpr int AT_ONCE = 32 / PIECES;           // rows copied per step
@@ -1038,11 +1056,12 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
       const int c = lane % PIECES, sub = lane / PIECES;
       const T* pool = reinterpret_cast<const T*>(keys ? p.k_pool : p.v_pool) + c * 8;
       const CUtensorMap* map = keys ? &k_map : &v_map;
+      const uint32_t stages = keys ? K7_K_STAGES : K7_V_STAGES;
       const uint32_t area = base + (keys ? S::K : S::V);
       const uint32_t full = base + (keys ? S::K_FULL : S::V_FULL), empty = base + (keys ? S::K_EMPTY : S::V_EMPTY);
       auto show = [&](const K7Piece& y, uint32_t index, bool there) {  // to the softmax warps
         if (keys && lane == 0) {
-          cards[index % K7_CARDS] = K7Card{y.len, y.tile, there ? y.n : 0, y.rows, y.item, y.prefix ? 1 : 0};
+          cards[index % K7_CARDS] = K7Card{y.len, y.tile, there ? y.n : 0, y.rows, y.item, y.prefix ? 1 : 0, y.seq0, y.row0, y.kv_head};
           mbar_arrive(base + S::CARD_FULL + (index % K7_CARDS) * 8);
         }
       };
@@ -1055,30 +1074,17 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
       show(x, 0, there);
       if (there) pages = k7_open_pages(p, x, x.tile * K7_KEYS, lane);
       while (there && ok) {
-        if (keys && piece >= 2 && !mbar_wait(base + S::Q_EMPTY + (piece & 1u) * 8, ((piece >> 1) - 1) & 1u)) {
-          k7_raise(p.status, TOME_DEV_TIMEOUT);
-          ok = false;
-          break;
-        }
-        for (int i = sub; keys && i < x.rows; i += AT_ONCE) {  // the queries come with the first keys
-          const int32_t row = x.row0 + i, s = row / p.ratio;
-          const T* src = reinterpret_cast<const T*>(p.q) + (x.seq0 + s) * p.q_stride +
-                         static_cast<int64_t>(x.kv_head * p.ratio + (row - s * p.ratio)) * D + c * 8;
-          k7_copy16(base + S::Q + (piece & 1u) * S::Q_BYTES + (c >> 3) * (K7_ROWS * 128) + i * 128 +
-                        (((c & 7) ^ (i & 7)) << 4),
-                    src, true);
-        }
         K7Piece next = x;
         K7Pages next_pages = {};
         bool next_there = false;
         for (int32_t j = 0; j < x.n; ++j, ++t) {
-          const uint32_t stage = t % K7_STAGES;
+          const uint32_t stage = t % stages;
           if (j + 1 == x.n) {  // the piece behind is looked up while this one's loads are under way
             next_there = k7_next<true>(p, pl, next, true, at, last);
             show(next, piece + 1, next_there);
             if (next_there) next_pages = k7_open_pages(p, next, next.tile * K7_KEYS, lane);
           }
-          if (t >= K7_STAGES && !mbar_wait(empty + stage * 8, (t / K7_STAGES - 1) & 1u)) {
+          if (t >= stages && !mbar_wait(empty + stage * 8, (t / stages - 1) & 1u)) {
             k7_raise(p.status, TOME_DEV_TIMEOUT);
             ok = false;
             break;
@@ -1096,7 +1102,6 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
               row = (page * p.kv_heads + x.kv_head) * p.block_size + (group - blk * p.block_size);
             whole = __all_sync(0xffffffffu, row >= 0);
           }
-          // (a piece's queries come by asynchronous copies, which every lane's arrival waits for)
           if (whole) {
             if (by_hand >> stage & 1u) {  // ordinary writes before the tensor copies'
               fence_proxy_async();
@@ -1140,13 +1145,13 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
     fence_proxy_async();  // the space is filled by tensor copies again
     tc_fence_before_sync();
     __syncthreads();
-    if (warp == K7_QK_WARP) {
+    if (warp == K7_ISSUE_WARP) {
       tc_fence_after_sync();
       tmem_dealloc(tmem, S::TMEM_COLS);
     }
   }
 
-  if (warp == K7_PV_WARP) {
+  if (warp == K7_WARPS - 1) {
     // For the joining kernel, dealt over the CTAs: where a row's pieces lie.
     for (int64_t i = blockIdx.x * 32 + lane; i < static_cast<int64_t>(p.n_seq) * p.heads; i += gridDim.x * 32) {
       const int32_t b = static_cast<int32_t>(i / p.heads), h = static_cast<int32_t>(i - static_cast<int64_t>(b) * p.heads);
@@ -1428,12 +1433,14 @@ extern "C" int32_t tome_shared_prefix_attention(
   p.prefix_blocks = prefix_blocks;
   p.seq_blocks = max_blocks;
   p.num_blocks = num_blocks;
-  // key / block_size for keys below 2^31: with s = ceil(log2 d), (2^(31+s) / d + 1) fits 32 bits
-  // and its product with the key, shifted back, is exact
-  int s = 0;
-  while ((1ll << s) < block_size) ++s;
-  p.div_shift = 31 + s;
-  p.div_magic = static_cast<uint32_t>((1ull << (31 + s)) / static_cast<uint64_t>(block_size) + 1);
+  auto divisor = [](int32_t d, uint32_t* magic, int32_t* shift) {
+    int s = 0;
+    while ((1ll << s) < d) ++s;
+    *shift = 31 + s;
+    *magic = static_cast<uint32_t>((1ull << (31 + s)) / static_cast<uint64_t>(d) + 1);
+  };
+  divisor(block_size, &p.div_magic, &p.div_shift);
+  divisor(p.ratio, &p.ratio_magic, &p.ratio_shift);
   p.c = scale * LOG2E;
   p.whole_pages = block_size % 16 == 0 && num_blocks > 0;
   p.ctas = std::max(1, std::min(info.sm_count, K7_MAX_CTAS));
