@@ -23,7 +23,10 @@
 
 namespace tome {
 
-constexpr int K6_THREADS = 256;
+#ifndef K6_CFG_THREADS
+#define K6_CFG_THREADS 128
+#endif
+constexpr int K6_THREADS = K6_CFG_THREADS;
 constexpr int K6_MAX_DIM = 256;
 
 struct K6Params {
@@ -59,9 +62,12 @@ __device__ __forceinline__ void k6_raise(int32_t* status, int32_t bit) {
 }
 
 // ------------------------------------------------------------------ eight elements <-> fp32
+// (pairs, for the packed fp32 arithmetic: two elements per instruction)
 struct K6Eight {
-  float v[8];
+  float2 v[4];
 };
+__device__ __forceinline__ float2 k6_both(float x) { return make_float2(x, x); }
+__device__ __forceinline__ float2 k6_neg(float2 x) { return make_float2(-x.x, -x.y); }
 
 template <typename T>
 struct K6Raw {  // eight elements as they sit in memory
@@ -115,17 +121,15 @@ template <typename T>
 __device__ __forceinline__ K6Eight k6_unpack(const K6Raw<T>& r) {
   K6Eight e;
   if constexpr (sizeof(T) == 4) {
-    const uint32_t w[8] = {r.a.x, r.a.y, r.a.z, r.a.w, r.b.x, r.b.y, r.b.z, r.b.w};
-#pragma unroll
-    for (int i = 0; i < 8; ++i) e.v[i] = __uint_as_float(w[i]);
+    e.v[0] = make_float2(__uint_as_float(r.a.x), __uint_as_float(r.a.y));
+    e.v[1] = make_float2(__uint_as_float(r.a.z), __uint_as_float(r.a.w));
+    e.v[2] = make_float2(__uint_as_float(r.b.x), __uint_as_float(r.b.y));
+    e.v[3] = make_float2(__uint_as_float(r.b.z), __uint_as_float(r.b.w));
   } else {
-    const uint32_t w[4] = {r.a.x, r.a.y, r.a.z, r.a.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const float2 f = k6_pair(w[i], T());
-      e.v[2 * i] = f.x;
-      e.v[2 * i + 1] = f.y;
-    }
+    e.v[0] = k6_pair(r.a.x, T());
+    e.v[1] = k6_pair(r.a.y, T());
+    e.v[2] = k6_pair(r.a.z, T());
+    e.v[3] = k6_pair(r.a.w, T());
   }
   return e;
 }
@@ -134,17 +138,24 @@ template <typename T>
 __device__ __forceinline__ K6Raw<T> k6_pack8(const K6Eight& e) {
   K6Raw<T> r;
   if constexpr (sizeof(T) == 4) {
-    r.a = make_uint4(__float_as_uint(e.v[0]), __float_as_uint(e.v[1]), __float_as_uint(e.v[2]),
-                     __float_as_uint(e.v[3]));
-    r.b = make_uint4(__float_as_uint(e.v[4]), __float_as_uint(e.v[5]), __float_as_uint(e.v[6]),
-                     __float_as_uint(e.v[7]));
+    r.a = make_uint4(__float_as_uint(e.v[0].x), __float_as_uint(e.v[0].y), __float_as_uint(e.v[1].x),
+                     __float_as_uint(e.v[1].y));
+    r.b = make_uint4(__float_as_uint(e.v[2].x), __float_as_uint(e.v[2].y), __float_as_uint(e.v[3].x),
+                     __float_as_uint(e.v[3].y));
   } else {
-    r.a = make_uint4(k6_pack(make_float2(e.v[0], e.v[1]), T()),
-                     k6_pack(make_float2(e.v[2], e.v[3]), T()),
-                     k6_pack(make_float2(e.v[4], e.v[5]), T()),
-                     k6_pack(make_float2(e.v[6], e.v[7]), T()));
+    r.a = make_uint4(k6_pack(e.v[0], T()), k6_pack(e.v[1], T()), k6_pack(e.v[2], T()), k6_pack(e.v[3], T()));
   }
   return r;
+}
+
+// Sum of the squares of a thread's sixteen elements.
+__device__ __forceinline__ float k6_squares(const K6Eight& a, const K6Eight& b) {
+  float2 s = __fmul2_rn(a.v[0], a.v[0]);
+#pragma unroll
+  for (int e = 1; e < 4; ++e) s = __ffma2_rn(a.v[e], a.v[e], s);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) s = __ffma2_rn(b.v[e], b.v[e], s);
+  return s.x + s.y;
 }
 
 __device__ __forceinline__ K6Eight k6_eight(const float* p) { return k6_unpack(k6_load_cached(p)); }
@@ -157,11 +168,38 @@ __device__ __forceinline__ float k6_group_sum(float x) {
   return x;
 }
 
+// Token and slot of item (first + i), i < 2^16: the quotient of the block's first item is the same for
+// all its threads, the rest is small.
+struct K6Place {
+  int64_t token;
+  int32_t slot;
+};
+__device__ __forceinline__ K6Place k6_place(int64_t first, int32_t i, int32_t per_token) {
+  const int64_t t0 = (first >> 31) == 0
+                         ? static_cast<int64_t>(static_cast<uint32_t>(first) / static_cast<uint32_t>(per_token))
+                         : first / per_token;
+  const uint32_t rest = static_cast<uint32_t>(first - t0 * per_token) + static_cast<uint32_t>(i);
+  const uint32_t q = rest / static_cast<uint32_t>(per_token);
+  return K6Place{t0 + q, static_cast<int32_t>(rest - q * per_token)};
+}
+
 // ------------------------------------------------------------------ forward and append
 // Work items of a token: ceil(heads / HPG) of queries, ceil(kv_heads / HPG) of keys and, when
 // appending, as many of values (copied).  G threads share a head.
+#ifndef K6_F_MINB
+#define K6_F_MINB 5
+#endif
+#ifndef K6_F_HPG
+#define K6_F_HPG 4
+#endif
+#ifndef K6_B_MINB
+#define K6_B_MINB 4
+#endif
+#ifndef K6_B_HPG
+#define K6_B_HPG 2
+#endif
 template <typename T, int G, int HPG>
-__global__ void __launch_bounds__(K6_THREADS) k6_forward_kernel(const K6Params p) {
+__global__ void __launch_bounds__(K6_THREADS, HPG == 1 ? 3 : (sizeof(T) == 4 ? 1 : K6_F_MINB)) k6_forward_kernel(const K6Params p) {
   const int j = threadIdx.x % G;  // which eight elements of a half
   const int half = p.dim >> 1;
   const bool on = j * 8 < half;   // groups are a power of two: some threads may have no elements
@@ -175,8 +213,9 @@ __global__ void __launch_bounds__(K6_THREADS) k6_forward_kernel(const K6Params p
   for (int64_t item = static_cast<int64_t>(blockIdx.x) * (K6_THREADS / G) + threadIdx.x / G;
        item < rounded; item += groups) {
     const bool live = on && item < items;
-    const int64_t t = live ? item / per_token : 0;
-    int slot = static_cast<int>(item - t * per_token);
+    const K6Place at_item = k6_place(item - threadIdx.x / G, threadIdx.x / G, per_token);
+    const int64_t t = live ? at_item.token : 0;
+    int slot = at_item.slot;
     const int kind = slot < q_items ? 0 : (slot < q_items + k_items ? 1 : 2);
     slot -= kind == 0 ? 0 : (kind == 1 ? q_items : q_items + k_items);
     const int h0 = slot * HPG;
@@ -247,18 +286,16 @@ __global__ void __launch_bounds__(K6_THREADS) k6_forward_kernel(const K6Params p
         a = k6_unpack(lo[i]);
         b = k6_unpack(hi[i]);
       }
-      float ss = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(a.v[e], a.v[e], fmaf(b.v[e], b.v[e], ss));
-      ss = k6_group_sum<G>(ss);
+      const float ss = k6_group_sum<G>(k6_squares(a, b));
       float r = rsqrtf(fmaf(ss, inv_dim, p.eps));
       if (bad) r = __int_as_float(0x7fc00000);
       K6Eight za, zb;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float ya = a.v[e] * r * w_lo.v[e], yb = b.v[e] * r * w_hi.v[e];
-        za.v[e] = ya * co.v[e] - yb * si.v[e];
-        zb.v[e] = yb * co.v[e] + ya * si.v[e];
+      for (int e = 0; e < 4; ++e) {
+        const float2 ya = __fmul2_rn(__fmul2_rn(a.v[e], k6_both(r)), w_lo.v[e]);
+        const float2 yb = __fmul2_rn(__fmul2_rn(b.v[e], k6_both(r)), w_hi.v[e]);
+        za.v[e] = __ffma2_rn(ya, co.v[e], __fmul2_rn(k6_neg(yb), si.v[e]));
+        zb.v[e] = __ffma2_rn(yb, co.v[e], __fmul2_rn(ya, si.v[e]));
       }
       // a key whose position is bad is not cached
       if (i < n && kind != 2 && dst != nullptr && !(bad && kind == 1 && p.k_out == nullptr)) {
@@ -270,134 +307,136 @@ __global__ void __launch_bounds__(K6_THREADS) k6_forward_kernel(const K6Params p
 }
 
 // ------------------------------------------------------------------ backward
-// Same items (queries, keys, values).  Each thread sums its elements' weight gradients over
-// all its heads; a block adds its groups' sums in a fixed order and leaves them in `partial`,
-// which k6_weight_grad_kernel adds over the blocks: the result does not depend on timing.
+// One kind of heads at a time, queries, then keys, then the values' copy: each thread sums the weight
+// gradients of its elements over all its heads of a kind, a block adds its groups' sums in a fixed
+// order and leaves them in `partial`, which k6_weight_grad_kernel adds over the blocks: the result
+// does not depend on timing.
 template <typename T, int G, int HPG>
-__global__ void __launch_bounds__(K6_THREADS) k6_backward_kernel(const K6Params p) {
+__global__ void __launch_bounds__(K6_THREADS, sizeof(T) == 4 ? 1 : K6_B_MINB) k6_backward_kernel(const K6Params p) {
   const int j = threadIdx.x % G;
   const int half = p.dim >> 1;
   const bool on = j * 8 < half;
-  const int64_t groups = static_cast<int64_t>(gridDim.x) * (K6_THREADS / G);
-  const int q_items = (p.heads + HPG - 1) / HPG, k_items = (p.kv_heads + HPG - 1) / HPG;
-  const int per_token = q_items + 2 * k_items;
-  const int64_t items = p.tokens * per_token;
+  constexpr int PER_BLOCK = K6_THREADS / G;
   const int64_t width = static_cast<int64_t>(p.heads + 2 * p.kv_heads) * p.dim;
   const float inv_dim = 1.0f / static_cast<float>(p.dim);
-  const int64_t rounded = (items + 32 / G - 1) / (32 / G) * (32 / G);
-  float dw[2][16];
-#pragma unroll
-  for (int i = 0; i < 16; ++i) dw[0][i] = dw[1][i] = 0.0f;
+  __shared__ float sums[K6_THREADS / 32][2][K6_MAX_DIM];
+  griddep_launch_dependents();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
-  for (int64_t item = static_cast<int64_t>(blockIdx.x) * (K6_THREADS / G) + threadIdx.x / G;
-       item < rounded; item += groups) {
-    const bool live = on && item < items;
-    const int64_t t = live ? item / per_token : 0;
-    int slot = static_cast<int>(item - t * per_token);
-    const int kind = slot < q_items ? 0 : (slot < q_items + k_items ? 1 : 2);
-    slot -= kind == 0 ? 0 : (kind == 1 ? q_items : q_items + k_items);
-    const int h0 = slot * HPG;
-    const int n = live ? min(HPG, (kind == 0 ? p.heads : p.kv_heads) - h0) : 0;
-    const int64_t column =
-        static_cast<int64_t>(h0 + (kind == 0 ? 0 : p.heads + (kind == 1 ? 0 : p.kv_heads))) * p.dim +
-        j * 8;
-    const T* x = reinterpret_cast<const T*>(p.qkv) + t * p.qkv_stride + column;
-    const T* g = kind == 0 ? reinterpret_cast<const T*>(p.grad_q) + (t * p.heads + h0) * p.dim + j * 8
-                           : reinterpret_cast<const T*>(kind == 1 ? p.grad_k : p.grad_v) +
-                                 (t * p.kv_heads + h0) * p.dim + j * 8;
-    T* dst = reinterpret_cast<T*>(p.grad_qkv) + t * width + column;
-    K6Raw<T> xl[HPG] = {}, xh[HPG] = {}, gl[HPG] = {}, gh[HPG] = {};
+#pragma unroll 1
+  for (int kind = 0; kind < 2; ++kind) {
+    const int heads = kind == 0 ? p.heads : p.kv_heads;
+    const int per_token = (heads + HPG - 1) / HPG;
+    const int64_t items = p.tokens * per_token;
+    const int64_t rounded = (items + 32 / G - 1) / (32 / G) * (32 / G);  // whole warps for the shuffles
+    const T* grads = reinterpret_cast<const T*>(kind == 0 ? p.grad_q : p.grad_k) + j * 8;
+    const int64_t column0 = (kind == 0 ? 0 : static_cast<int64_t>(p.heads) * p.dim) + j * 8;
+    K6Raw<T> w_lo = {}, w_hi = {};
+    if (on) {
+      const T* w = reinterpret_cast<const T*>(kind == 0 ? p.q_weight : p.k_weight) + j * 8;
+      w_lo = k6_load_cached(w);
+      w_hi = k6_load_cached(w + half);
+    }
+    float2 dw[8];
 #pragma unroll
-    for (int i = 0; i < HPG; ++i)
-      if (i < n) {
-        if (kind != 2) {
+    for (int i = 0; i < 8; ++i) dw[i] = make_float2(0.0f, 0.0f);
+    for (int64_t first = static_cast<int64_t>(blockIdx.x) * PER_BLOCK; first + threadIdx.x / G < rounded;
+         first += static_cast<int64_t>(gridDim.x) * PER_BLOCK) {
+      const K6Place at = k6_place(first, threadIdx.x / G, per_token);
+      const bool live = on && at.token < p.tokens;
+      const int64_t t = live ? at.token : 0;
+      const int h0 = at.slot * HPG;
+      const int n = live ? min(HPG, heads - h0) : 0;
+      const T* x = reinterpret_cast<const T*>(p.qkv) + t * p.qkv_stride + column0 + h0 * p.dim;
+      const T* g = grads + (t * heads + h0) * p.dim;
+      T* dst = reinterpret_cast<T*>(p.grad_qkv) + t * width + column0 + h0 * p.dim;
+      K6Raw<T> xl[HPG] = {}, xh[HPG] = {}, gl[HPG] = {}, gh[HPG] = {};
+#pragma unroll
+      for (int i = 0; i < HPG; ++i)
+        if (i < n) {
           xl[i] = k6_load(x + i * p.dim);
           xh[i] = k6_load(x + i * p.dim + half);
-        }
-        if (kind != 2 || p.grad_v != nullptr) {
           gl[i] = k6_load(g + i * p.dim);
           gh[i] = k6_load(g + i * p.dim + half);
         }
+      K6Eight co = {}, si = {};
+      bool bad = false;
+      if (n > 0) {
+        const int32_t pos = p.positions[t];
+        bad = pos < 0 || pos >= p.n_positions;
+        if (bad && j == 0) k6_raise(p.status, TOME_DEV_POSITION_OUT_OF_RANGE);
+        const float* cs = p.cos_sin + static_cast<int64_t>(bad ? 0 : pos) * p.dim + j * 8;
+        co = k6_eight(cs);
+        si = k6_eight(cs + half);
       }
-    K6Eight w_lo = {}, w_hi = {}, co = {}, si = {};
-    bool bad = false;
-    if (n > 0 && kind != 2) {
-      const T* w = reinterpret_cast<const T*>(kind == 0 ? p.q_weight : p.k_weight) + j * 8;
-      w_lo = k6_unpack(k6_load_cached(w));
-      w_hi = k6_unpack(k6_load_cached(w + half));
-      const int32_t pos = p.positions[t];
-      bad = pos < 0 || pos >= p.n_positions;
-      if (bad && j == 0) k6_raise(p.status, TOME_DEV_POSITION_OUT_OF_RANGE);
-      const float* cs = p.cos_sin + static_cast<int64_t>(bad ? 0 : pos) * p.dim + j * 8;
-      co = k6_eight(cs);
-      si = k6_eight(cs + half);
-    }
-    const float q_on = kind == 0 ? 1.0f : 0.0f, k_on = kind == 1 ? 1.0f : 0.0f;
 #pragma unroll
-    for (int i = 0; i < HPG; ++i) {
-      const K6Eight a = k6_unpack(xl[i]), b = k6_unpack(xh[i]);
-      const K6Eight da = k6_unpack(gl[i]), db = k6_unpack(gh[i]);
-      float ss = 0.0f;
+      for (int i = 0; i < HPG; ++i) {
+        const K6Eight a = k6_unpack(xl[i]), b = k6_unpack(xh[i]);
+        const float ss = k6_group_sum<G>(k6_squares(a, b));
+        float r = rsqrtf(fmaf(ss, inv_dim, p.eps));
+        if (bad) r = __int_as_float(0x7fc00000);
+        const K6Eight da = k6_unpack(gl[i]), db = k6_unpack(gh[i]), wa = k6_unpack(w_lo), wb = k6_unpack(w_hi);
+        K6Eight ya, yb;  // gradient of the normed head (rotation turned back), times the weight
+        float2 dot2 = make_float2(0.0f, 0.0f);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(a.v[e], a.v[e], fmaf(b.v[e], b.v[e], ss));
-      ss = k6_group_sum<G>(ss);
-      float r = rsqrtf(fmaf(ss, inv_dim, p.eps));
-      if (bad) r = __int_as_float(0x7fc00000);
-      K6Eight ya, yb;  // gradient of the normed head (rotation turned back)
-      float dot = 0.0f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ya.v[e] = da.v[e] * co.v[e] + db.v[e] * si.v[e];
-        yb.v[e] = db.v[e] * co.v[e] - da.v[e] * si.v[e];
-        const float na = a.v[e] * r, nb = b.v[e] * r;
-        if (i < n && kind != 2) {
-          const float ca = ya.v[e] * na, cb = yb.v[e] * nb;
-          dw[0][e] = fmaf(q_on, ca, dw[0][e]);
-          dw[0][8 + e] = fmaf(q_on, cb, dw[0][8 + e]);
-          dw[1][e] = fmaf(k_on, ca, dw[1][e]);
-          dw[1][8 + e] = fmaf(k_on, cb, dw[1][8 + e]);
+        for (int e = 0; e < 4; ++e) {
+          const float2 na = __fmul2_rn(a.v[e], k6_both(r)), nb = __fmul2_rn(b.v[e], k6_both(r));
+          ya.v[e] = __ffma2_rn(da.v[e], co.v[e], __fmul2_rn(db.v[e], si.v[e]));
+          yb.v[e] = __ffma2_rn(db.v[e], co.v[e], __fmul2_rn(k6_neg(da.v[e]), si.v[e]));
+          dw[e] = __ffma2_rn(ya.v[e], na, dw[e]);  // (heads that are not there have zeros)
+          dw[4 + e] = __ffma2_rn(yb.v[e], nb, dw[4 + e]);
+          ya.v[e] = __fmul2_rn(ya.v[e], wa.v[e]);
+          yb.v[e] = __fmul2_rn(yb.v[e], wb.v[e]);
+          dot2 = __ffma2_rn(ya.v[e], na, __ffma2_rn(yb.v[e], nb, dot2));
         }
-        ya.v[e] *= w_lo.v[e];
-        yb.v[e] *= w_hi.v[e];
-        dot = fmaf(ya.v[e], na, fmaf(yb.v[e], nb, dot));
-      }
-      dot = k6_group_sum<G>(dot) * inv_dim;
+        const float dot = -k6_group_sum<G>(dot2.x + dot2.y) * inv_dim * r;
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ya.v[e] = r * (ya.v[e] - a.v[e] * r * dot);
-        yb.v[e] = r * (yb.v[e] - b.v[e] * r * dot);
-      }
-      if (i < n) {
-        k6_store(dst + i * p.dim, kind == 2 ? gl[i] : k6_pack8<T>(ya));
-        k6_store(dst + i * p.dim + half, kind == 2 ? gh[i] : k6_pack8<T>(yb));
+        for (int e = 0; e < 4; ++e) {
+          ya.v[e] = __fmul2_rn(k6_both(r), __ffma2_rn(a.v[e], k6_both(dot), ya.v[e]));
+          yb.v[e] = __fmul2_rn(k6_both(r), __ffma2_rn(b.v[e], k6_both(dot), yb.v[e]));
+        }
+        if (i < n) {
+          k6_store(dst + i * p.dim, k6_pack8<T>(ya));
+          k6_store(dst + i * p.dim + half, k6_pack8<T>(yb));
+        }
       }
     }
-  }
-
-  // the block's sums, group after group
-  __shared__ float sums[2][K6_MAX_DIM];
-  for (int i = threadIdx.x; i < 2 * K6_MAX_DIM; i += K6_THREADS) (&sums[0][0])[i] = 0.0f;
-  // first over the groups of a warp (lanes that differ in their group's bits), then over warps
+    // the warp's sums, over its groups (lanes that differ in their group's bits)
 #pragma unroll
-  for (int s = 0; s < 2; ++s)
+    for (int e = 0; e < 8; ++e)
 #pragma unroll
-    for (int e = 0; e < 16; ++e)
+      for (int o = 16; o >= G; o >>= 1) {
+        dw[e].x += __shfl_xor_sync(0xffffffffu, dw[e].x, o);
+        dw[e].y += __shfl_xor_sync(0xffffffffu, dw[e].y, o);
+      }
+    if (lane < G && on)
 #pragma unroll
-      for (int o = 16; o >= G; o >>= 1) dw[s][e] += __shfl_xor_sync(0xffffffffu, dw[s][e], o);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  for (int w = 0; w < K6_THREADS / 32; ++w) {
-    __syncthreads();
-    if (warp == w && lane < G && on)
-      for (int e = 0; e < 8; ++e)
-        for (int s = 0; s < 2; ++s) {
-          sums[s][j * 8 + e] += dw[s][e];
-          sums[s][half + j * 8 + e] += dw[s][8 + e];
-        }
+      for (int e = 0; e < 4; ++e) {
+        *reinterpret_cast<float2*>(&sums[warp][kind][j * 8 + 2 * e]) = dw[e];
+        *reinterpret_cast<float2*>(&sums[warp][kind][half + j * 8 + 2 * e]) = dw[4 + e];
+      }
   }
   __syncthreads();
-  for (int i = threadIdx.x; i < 2 * p.dim; i += K6_THREADS)
-    p.partial[static_cast<int64_t>(blockIdx.x) * 2 * p.dim + i] =
-        sums[i / p.dim][i - (i / p.dim) * p.dim];
+  for (int i = threadIdx.x; i < 2 * p.dim; i += K6_THREADS) {
+    const int kind = i >= p.dim, e = i - kind * p.dim;
+    float s = 0.0f;
+#pragma unroll
+    for (int w = 0; w < K6_THREADS / 32; ++w) s += sums[w][kind][e];
+    p.partial[static_cast<int64_t>(blockIdx.x) * 2 * p.dim + i] = s;
+  }
+
+  // the values' part: copied, or zeros
+  constexpr int ES = 16 / sizeof(T);
+  const int64_t per_token = static_cast<int64_t>(p.kv_heads) * p.dim / ES, all = p.tokens * per_token;
+  const int64_t step = static_cast<int64_t>(gridDim.x) * K6_THREADS;
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * K6_THREADS + threadIdx.x; i < all; i += step) {
+    const int64_t t = (i >> 31) == 0 ? static_cast<int64_t>(static_cast<uint32_t>(i) / static_cast<uint32_t>(per_token))
+                                     : i / per_token;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    if (p.grad_v != nullptr) v = __ldcs(reinterpret_cast<const uint4*>(p.grad_v) + i);
+    stg128_streaming(reinterpret_cast<T*>(p.grad_qkv) + t * width + static_cast<int64_t>(p.heads + p.kv_heads) * p.dim +
+                         (i - t * per_token) * ES, v);
+  }
 }
 
 // out[i] = sum over the blocks of partial[block, i], i < 2 * dim: 32 columns per block, the
@@ -486,23 +525,26 @@ static int32_t k6_launch(const K6Params& p, int32_t dtype, cudaStream_t stream, 
   const int64_t heads_in_all = p.tokens * (p.heads + sections * p.kv_heads);
   // One head per group while that still fills no more than the device once (a decode step:
   // latency), else several heads of a token share its cos and sin.
-  const int many = BACK ? 2 : 4;
+  const int many = BACK ? K6_B_HPG : K6_F_HPG;
   const bool one = heads_in_all <= static_cast<int64_t>(info.sm_count) * 2 * per_block;
   const int hpg = one ? 1 : many;
   const int64_t items =
       p.tokens * ((p.heads + hpg - 1) / hpg + sections * ((p.kv_heads + hpg - 1) / hpg));
   const int64_t want = (items + per_block - 1) / per_block;
   int64_t blocks = std::max<int64_t>(1, want);
-  if (BACK) blocks = std::min<int64_t>(blocks, std::min(info.sm_count * 2, K6_MAX_BLOCKS));
+#ifndef K6_B_GRID
+#define K6_B_GRID 4
+#endif
+  if (BACK) blocks = std::min<int64_t>(blocks, std::min(info.sm_count * K6_B_GRID, K6_MAX_BLOCKS));
   else blocks = std::min<int64_t>(blocks, static_cast<int64_t>(1) << 30);
   const void* kernel = nullptr;
   if (dtype == TOME_F32)
-    kernel = one ? k6_kernel_of<float, 1, BACK>(g) : k6_kernel_of<float, BACK ? 2 : 4, BACK>(g);
+    kernel = one ? k6_kernel_of<float, 1, BACK>(g) : k6_kernel_of<float, BACK ? K6_B_HPG : K6_F_HPG, BACK>(g);
   else if (dtype == TOME_BF16)
     kernel = one ? k6_kernel_of<__nv_bfloat16, 1, BACK>(g)
-                 : k6_kernel_of<__nv_bfloat16, BACK ? 2 : 4, BACK>(g);
+                 : k6_kernel_of<__nv_bfloat16, BACK ? K6_B_HPG : K6_F_HPG, BACK>(g);
   else
-    kernel = one ? k6_kernel_of<__half, 1, BACK>(g) : k6_kernel_of<__half, BACK ? 2 : 4, BACK>(g);
+    kernel = one ? k6_kernel_of<__half, 1, BACK>(g) : k6_kernel_of<__half, BACK ? K6_B_HPG : K6_F_HPG, BACK>(g);
   void* args[] = {const_cast<K6Params*>(&p)};
   if (blocks_out != nullptr) *blocks_out = static_cast<int>(blocks);
   return check_cuda(cudaLaunchKernel(kernel, dim3(static_cast<unsigned>(blocks)), dim3(K6_THREADS),
@@ -637,6 +679,11 @@ extern "C" int32_t tome_qk_norm_rope_backward(
   cfg.gridDim = dim3(static_cast<unsigned>((2 * head_dim + 31) / 32));
   cfg.blockDim = dim3(1024);
   cfg.stream = static_cast<cudaStream_t>(stream);
+  cudaLaunchAttribute attr;  // set up while the kernel before drains
+  attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
   return check_cuda(cudaLaunchKernelEx(&cfg, k6_weight_grad_kernel,
                                        static_cast<const float*>(p.partial), blocks, head_dim,
                                        grad_q_weight, grad_k_weight),
