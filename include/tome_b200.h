@@ -448,12 +448,9 @@ int32_t tome_shared_prefix_attention(const void* q, int32_t dtype, int64_t n_seq
  *   out_loss   device fp32 [1]; out_logprob device fp32 [n_seq * seq_len], 0 outside the windows
  *   out_grad   device, shape and type of logits, contiguous, 16-byte aligned, not overlapping
  *              them; zeros outside the windows.  NULL: the loss alone, the logits read once
- *   workspace  device scratch of tome_grpo_policy_loss_workspace_bytes, 16-byte aligned; needs no
- *              initialisation
  * Rows outside the windows are never read.  A target outside [0, vocab) makes its row and the
  * loss NaN and sets TOME_DEV_TARGET_OUT_OF_RANGE.  The sums do not depend on timing.
  */
-size_t tome_grpo_policy_loss_workspace_bytes(int64_t n_seq, int64_t seq_len);
 int32_t tome_grpo_policy_loss(const void* logits, int32_t dtype, int64_t n_seq, int64_t seq_len,
                               int64_t vocab, const int32_t* targets, const float* old_logprob,
                               const float* ref_logprob, const float* advantages,
@@ -461,8 +458,7 @@ int32_t tome_grpo_policy_loss(const void* logits, int32_t dtype, int64_t n_seq, 
                               const int32_t* starts, float temperature, float clip_low,
                               float clip_high, float kl_coef, int32_t per_sequence,
                               float grad_scale, float* out_loss, float* out_logprob,
-                              void* out_grad, void* workspace, size_t workspace_bytes,
-                              int32_t* dev_status, void* stream);
+                              void* out_grad, int32_t* dev_status, void* stream);
 
 #ifdef __cplusplus
 }

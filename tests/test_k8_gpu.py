@@ -198,8 +198,7 @@ def test_repetition_streams_graphs_and_out(cuda_device):
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(call(), held))
     for kw in ({"out_grad": dev["logits"]}, {"out_grad": out.float()}, {"out_grad": out[:1]}, {"reduction": "sum"},
-               {"out_grad": out, "return_grad": False}, {"clip_low": -1.0}, {"grad_scale": float("nan")},
-               {"workspace": torch.zeros(4, dtype=torch.uint8, device=cuda_device)}):
+               {"out_grad": out, "return_grad": False}, {"clip_low": -1.0}, {"grad_scale": float("nan")}):
         with pytest.raises((ValueError, TypeError)):
             call(**kw)
     with pytest.raises(ValueError):

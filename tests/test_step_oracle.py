@@ -150,13 +150,11 @@ def test_attention_refusals(built_lib):
 def test_policy_loss_refusals(built_lib):
     from tome_b200 import _lib
     lib, p, odd = _lib.lib, ctypes.c_void_p(0x1000), ctypes.c_void_p(0x1008)
-    need = lib.tome_grpo_policy_loss_workspace_bytes(3, 5)
-    assert need >= 60 and lib.tome_grpo_policy_loss_workspace_bytes(0, 5) == 0
 
     def loss(lg=p, dtype=1, n=3, length=5, vocab=64, ids=p, old=p, ref=p, adv=p, temp=1.0, low=0.2, high=0.2,
-             beta=0.1, scale=1.0, out=p, lp=p, grad=p, ws=p, size=need):
+             beta=0.1, scale=1.0, out=p, lp=p, grad=p):
         return lib.tome_grpo_policy_loss(lg, dtype, n, length, vocab, ids, old, ref, adv, 0, p, None, temp, low, high,
-                                         beta, 0, scale, out, lp, grad, ws, size, None, None)
+                                         beta, 0, scale, out, lp, grad, None, None)
     assert loss(dtype=2) == -3 and loss(dtype=-1) == -3
     assert loss(n=-1) == -4 and loss(vocab=0) == -4 and loss(length=-2) == -4
     assert loss(temp=0.0) == -7 and loss(temp=float("nan")) == -7
@@ -164,8 +162,7 @@ def test_policy_loss_refusals(built_lib):
     assert loss(scale=float("inf")) == -4
     assert loss(out=None) == -1 and loss(lg=None) == -1 and loss(ids=None) == -1 and loss(old=None) == -1
     assert loss(adv=None) == -1 and loss(lp=None) == -1 and loss(ref=None) == -1
-    assert loss(lg=odd) == -2 and loss(grad=odd) == -2 and loss(ws=odd) == -2
-    assert loss(ws=None) == -6 and loss(size=need - 1) == -6
+    assert loss(lg=odd) == -2 and loss(grad=odd) == -2
 
 
 def test_cpu_tensors_are_refused(built_lib):

@@ -24,12 +24,11 @@ __all__ = _OPS + _DIST + _LIB
 
 
 def __getattr__(name):
-    if name in _OPS:
-        return getattr(importlib.import_module(".ops", __name__), name)
-    if name in _DIST:
-        return getattr(importlib.import_module(".dist", __name__), name)
-    if name in _LIB:
-        return getattr(importlib.import_module("._lib", __name__), name)
+    for names, module in ((_OPS, ".ops"), (_DIST, ".dist"), (_LIB, "._lib")):
+        if name in names:
+            value = getattr(importlib.import_module(module, __name__), name)
+            globals()[name] = value  # looked up once: this function takes microseconds
+            return value
     if name in ("ops", "dist", "_lib", "synthetic", "build"):
         return importlib.import_module("." + name, __name__)
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -87,12 +87,10 @@ SIGNATURES = {
         c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_int32,
                   c_int32, c_void_p, c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_void_p,
                   c_int32, c_float, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
-    "tome_grpo_policy_loss_workspace_bytes": (
-        c_size_t, [c_int64, c_int64]),
     "tome_grpo_policy_loss": (
         c_int32, [c_void_p, c_int32, c_int64, c_int64, c_int64, c_void_p, c_void_p, c_void_p, c_void_p, c_int32,
                   c_void_p, c_void_p, c_float, c_float, c_float, c_float, c_int32, c_float,
-                  c_void_p, c_void_p, c_void_p, c_void_p, c_size_t, c_void_p, c_void_p]),
+                  c_void_p, c_void_p, c_void_p, c_void_p, c_void_p]),
     "tome_combine_triples": (c_int32, [c_void_p, c_void_p, c_int64, c_int32, c_void_p, c_int64,
                                        c_int32, c_int64, c_void_p, c_void_p, c_void_p]),
 }

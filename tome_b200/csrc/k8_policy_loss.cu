@@ -43,7 +43,6 @@ struct K8Params {
   float c, temp, inv_temp;  // log2(e)/T, T, 1/T
   float low, high, beta, scale;
   float* out_lp;            // [rows], 0 outside the windows
-  float* term;              // [rows] scratch: w l of each position
   float* out_loss;
   int32_t chunk_bytes;
   int32_t* status;
@@ -65,6 +64,25 @@ __device__ __forceinline__ void k8_window(const K8Params& p, int i, int& start, 
   start = (p.starts != nullptr) ? p.starts[i] : 0;
   start = max(0, min(start, p.seq_len));
   len = max(0, min(p.lengths[i], p.seq_len - start));
+}
+
+// The loss of a position from its log-prob, and its slope in it.
+struct K8Term {
+  float l, slope;
+};
+__device__ __forceinline__ K8Term k8_term(const K8Params& p, float lp, float old_lp, float ref_lp, float adv) {
+  const float rho = expf(lp - old_lp);
+  const float kept = fminf(fmaxf(rho, 1.0f - p.low), 1.0f + p.high);
+  const bool open = !(rho * adv > kept * adv);  // a NaN takes this branch and stays one
+  K8Term t;
+  t.l = open ? -(rho * adv) : -(kept * adv);
+  t.slope = open ? -(rho * adv) : 0.0f;
+  if (p.ref_lp != nullptr) {
+    const float d = ref_lp - lp, em = expm1f(d);
+    t.l = fmaf(p.beta, em - d, t.l);
+    t.slope = fmaf(-p.beta, em, t.slope);
+  }
+  return t;
 }
 
 // Eight (four) logits -> gradient, away from the target column: k * 2^((x - m) c), k = -slope / s.
@@ -138,6 +156,7 @@ k8_policy_loss_kernel(const K8Params p, const int cluster, const int chunks_per_
     if (lane == 0) *total_len = sum;
   }
   __syncthreads();
+  griddep_launch_dependents();
   if (cluster > 1) cluster_sync_all();  // nobody arrives on a barrier that is not there yet
 
   const int64_t bulk_most = (p.vocab * ES) & ~static_cast<int64_t>(15);
@@ -221,7 +240,6 @@ k8_policy_loss_kernel(const K8Params p, const int cluster, const int chunks_per_
         }
         if (rank == 0 && ctid == 0) {
           p.out_lp[row] = 0.0f;
-          p.term[row] = 0.0f;
         }
         continue;
       }
@@ -294,17 +312,7 @@ k8_policy_loss_kernel(const K8Params p, const int cluster, const int chunks_per_
           raise_status(p.status, TOME_DEV_TIMEOUT);
           lp = __int_as_float(0x7fc00000);
         }
-        // the loss of this position and its slope in lp
-        const float rho = expf(lp - old_lp);
-        const float kept = fminf(fmaxf(rho, 1.0f - p.low), 1.0f + p.high);
-        const bool open = !(rho * adv > kept * adv);  // a NaN takes this branch and stays one
-        float l = open ? -(rho * adv) : -(kept * adv);
-        float slope = open ? -(rho * adv) : 0.0f;
-        if (p.ref_lp != nullptr) {
-          const float d = ref_lp - lp, em = expm1f(d);
-          l = fmaf(p.beta, em - d, l);
-          slope = fmaf(-p.beta, em, slope);
-        }
+        const float slope = k8_term(p, lp, old_lp, ref_lp, adv).slope;
         const float weight =
             p.per_sequence ? 1.0f / (static_cast<float>(p.n_seq) * static_cast<float>(win_len))
                            : 1.0f / static_cast<float>(*total_len);
@@ -315,7 +323,6 @@ k8_policy_loss_kernel(const K8Params p, const int cluster, const int chunks_per_
           box[par].z = fmaf(-g / s, ex2f((x_t - m) * p.c), g);  // the target column's gradient
           if (rank == 0) {
             p.out_lp[row] = lp;
-            p.term[row] = l * weight;
             if (!target_ok) raise_status(p.status, TOME_DEV_TARGET_OUT_OF_RANGE);
           }
         }
@@ -361,21 +368,46 @@ k8_policy_loss_kernel(const K8Params p, const int cluster, const int chunks_per_
   if (cluster > 1) cluster_sync_all();
 }
 
-// loss = sum of the rows' terms, in 64 bits and in an order that depends on the sizes alone.
-__global__ void __launch_bounds__(1024) k8_sum_kernel(const float* term, int64_t rows, float* out) {
+// loss = sum of w l over the windows, from the log-probs that the kernel above left, in 64 bits and
+// in an order that depends on the sizes alone.
+__global__ void __launch_bounds__(1024) k8_sum_kernel(const K8Params p) {
   __shared__ double sums[32];
+  __shared__ int64_t counts[32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   griddep_wait();
   double s = 0.0;
-  for (int64_t i = threadIdx.x; i < rows; i += 1024) s += static_cast<double>(term[i]);
+  int64_t active = 0;
+  for (int64_t i = threadIdx.x; i < p.rows; i += 1024) {
+    const int seq = static_cast<int>(i / p.seq_len);
+    const int pos = static_cast<int>(i - static_cast<int64_t>(seq) * p.seq_len);
+    int st, ln;
+    k8_window(p, seq, st, ln);
+    if (pos < st || pos >= st + ln) continue;
+    const float l = k8_term(p, p.out_lp[i], p.old_lp[i], p.ref_lp != nullptr ? p.ref_lp[i] : 0.0f,
+                            p.advantages[p.adv_per_token ? i : seq]).l;
+    s += p.per_sequence ? static_cast<double>(l) / (static_cast<double>(p.n_seq) * ln) : static_cast<double>(l);
+    ++active;
+  }
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-  if ((threadIdx.x & 31) == 0) sums[threadIdx.x >> 5] = s;
+  for (int o = 16; o > 0; o >>= 1) {
+    s += __shfl_xor_sync(0xffffffffu, s, o);
+    active += __shfl_xor_sync(0xffffffffu, active, o);
+  }
+  if (lane == 0) {
+    sums[warp] = s;
+    counts[warp] = active;
+  }
   __syncthreads();
-  if (threadIdx.x < 32) {
-    s = sums[threadIdx.x];
+  if (warp == 0) {
+    s = sums[lane];
+    active = counts[lane];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) s += __shfl_xor_sync(0xffffffffu, s, o);
-    if (threadIdx.x == 0) *out = static_cast<float>(s);
+    for (int o = 16; o > 0; o >>= 1) {
+      s += __shfl_xor_sync(0xffffffffu, s, o);
+      active += __shfl_xor_sync(0xffffffffu, active, o);
+    }
+    if (lane == 0)
+      *p.out_loss = static_cast<float>(p.per_sequence || active == 0 ? s : s / static_cast<double>(active));
   }
 }
 
@@ -433,19 +465,17 @@ static int32_t k8_launch(K8Params p, int sm_count, cudaStream_t stream) {
   sum.gridDim = dim3(1);
   sum.blockDim = dim3(1024);
   sum.stream = stream;
-  return check_cuda(cudaLaunchKernelEx(&sum, k8_sum_kernel, static_cast<const float*>(p.term),
-                                       p.rows, p.out_loss),
-                    "policy loss sum launch");
+  cudaLaunchAttribute early;  // set up while the kernel before drains
+  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  early.val.programmaticStreamSerializationAllowed = 1;
+  sum.attrs = &early;
+  sum.numAttrs = 1;
+  return check_cuda(cudaLaunchKernelEx(&sum, k8_sum_kernel, p), "policy loss sum launch");
 }
 
 }  // namespace tome
 
 using namespace tome;
-
-extern "C" size_t tome_grpo_policy_loss_workspace_bytes(int64_t n_seq, int64_t seq_len) {
-  if (n_seq <= 0 || seq_len <= 0) return 0;
-  return static_cast<size_t>(n_seq) * static_cast<size_t>(seq_len) * sizeof(float);
-}
 
 extern "C" int32_t tome_grpo_policy_loss(
     const void* logits, int32_t dtype, int64_t n_seq, int64_t seq_len, int64_t vocab,
@@ -453,7 +483,7 @@ extern "C" int32_t tome_grpo_policy_loss(
     const float* advantages, int32_t advantage_per_token, const int32_t* lengths,
     const int32_t* starts, float temperature, float clip_low, float clip_high, float kl_coef,
     int32_t per_sequence, float grad_scale, float* out_loss, float* out_logprob, void* out_grad,
-    void* workspace, size_t workspace_bytes, int32_t* dev_status, void* stream) {
+    int32_t* dev_status, void* stream) {
   if (dtype != TOME_F32 && dtype != TOME_BF16) return fail(TOME_ERR_BAD_DTYPE, "dtype=%d", dtype);
   if (n_seq < 0 || seq_len < 0 || vocab <= 0 || n_seq > 0x7fffffff || seq_len > 0x7fffffff)
     return fail(TOME_ERR_BAD_SHAPE, "n_seq=%lld seq_len=%lld vocab=%lld", (long long)n_seq,
@@ -478,16 +508,12 @@ extern "C" int32_t tome_grpo_policy_loss(
       return fail(TOME_ERR_NULL_POINTER, "kl_coef=%g without ref_logprob", (double)kl_coef);
     if (!aligned16(logits) || (out_grad != nullptr && !aligned16(out_grad)))
       return fail(TOME_ERR_MISALIGNED, "logits and the gradient must be 16-byte aligned");
-    if (workspace == nullptr || workspace_bytes < tome_grpo_policy_loss_workspace_bytes(n_seq, seq_len))
-      return fail(TOME_ERR_WORKSPACE_TOO_SMALL, "workspace of %zu bytes, %zu needed", workspace_bytes,
-                  tome_grpo_policy_loss_workspace_bytes(n_seq, seq_len));
-    if (!aligned16(workspace)) return fail(TOME_ERR_MISALIGNED, "workspace must be 16-byte aligned");
   }
   DeviceInfo info;
   const int32_t st = current_device_info(&info);
   if (st != TOME_OK) return st;
   if (rows == 0) {
-    k8_sum_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(nullptr, 0, out_loss);
+    k8_sum_kernel<<<1, 1024, 0, static_cast<cudaStream_t>(stream)>>>(p);
     return check_cuda(cudaGetLastError(), "policy loss sum launch");
   }
   p.logits = logits;
@@ -511,7 +537,6 @@ extern "C" int32_t tome_grpo_policy_loss(
   p.beta = kl_coef;
   p.scale = grad_scale;
   p.out_lp = out_logprob;
-  p.term = static_cast<float*>(workspace);
   p.status = dev_status;
   if (dtype == TOME_F32) return k8_launch<float>(p, info.sm_count, static_cast<cudaStream_t>(stream));
   return k8_launch<__nv_bfloat16>(p, info.sm_count, static_cast<cudaStream_t>(stream));

@@ -846,6 +846,10 @@ def _ints(name: str, t: torch.Tensor, shape, device: torch.device) -> torch.Tens
     return t.to(device=device, dtype=torch.int32).contiguous()
 
 
+def _plain(t: torch.Tensor, dtype: torch.dtype, device: torch.device) -> bool:
+    return t.dtype is dtype and t.device == device and t.is_contiguous()
+
+
 def _index(ids: torch.Tensor, n: int, device: torch.device) -> torch.Tensor:
     """:func:`_ids32` for a tensor of any shape, without a call where nothing is to be done."""
     if isinstance(ids, torch.Tensor) and ids.dtype is torch.int32 and ids.device == device and \
@@ -884,6 +888,12 @@ def _out_tensor(name: str, t: Optional[torch.Tensor], shape, dtype: torch.dtype,
     if not t.is_contiguous() or t.data_ptr() % 16:
         raise ValueError(f"{name} must be contiguous and 16-byte aligned")
     return t
+
+
+def _all_tensors(**tensors) -> None:
+    for name, t in tensors.items():
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f"{name} must be a torch.Tensor, got {type(t).__name__}")
 
 
 def _span(t: torch.Tensor) -> Tuple[int, int]:
@@ -936,6 +946,18 @@ def _cached_bytes(query, *sizes) -> int:
 def _norm_rope_args(qkv, q_weight, k_weight, cos_sin, positions, heads, kv_heads):
     """Checked arguments that the three forms share: (rows of qkv, its stride, weights, table,
     positions, head_dim, dtype code)."""
+    if qkv.dim() == 2 and qkv.is_contiguous():  # nothing to convert, as a rule
+        n, width = qkv.shape
+        dtype, device, dim = qkv.dtype, qkv.device, q_weight.numel()
+        if (heads + 2 * kv_heads) * dim == width and dtype in _MODEL_DTYPES and heads > 0 and \
+                kv_heads > 0 and _plain(q_weight, dtype, device) and _plain(k_weight, dtype, device) and \
+                q_weight.dim() == 1 and k_weight.shape == q_weight.shape and \
+                _plain(cos_sin, torch.float32, device) and cos_sin.dim() == 2 and \
+                cos_sin.shape[1] == dim and positions.dtype is torch.int32 and \
+                positions.device == device and positions.numel() == n and positions.is_contiguous() and \
+                not (qkv.data_ptr() | q_weight.data_ptr() | k_weight.data_ptr() | cos_sin.data_ptr()) & 15 \
+                and width * qkv.element_size() % 16 == 0 and qkv.is_cuda:
+            return qkv, width, q_weight, k_weight, cos_sin, positions, dim, _MODEL_DTYPES[dtype]
     _require_cuda("qkv", qkv)
     if qkv.dtype not in _MODEL_DTYPES:
         raise TypeError(f"qkv must be float32, bfloat16 or float16, got {qkv.dtype}")
@@ -976,6 +998,9 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: torch.Tens
     :func:`qk_norm_rope_backward` is its gradient, :func:`qk_norm_rope_append` the form for
     decoding, which writes keys and values into the paged cache.
     """
+    _all_tensors(qkv=qkv, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin)
+    if not isinstance(positions, torch.Tensor):
+        positions = torch.as_tensor(positions)
     rows, stride, qw, kw, cs, pos, dim, code = _norm_rope_args(qkv, q_weight, k_weight, cos_sin,
                                                                positions, heads, kv_heads)
     device, n, lead = rows.device, rows.shape[0], tuple(qkv.shape[:-1])
@@ -1013,14 +1038,16 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
     or the pool does not have is skipped and reported through the device status; two tokens of
     a call must not name the same place.
     """
-    for name, t in (("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables)):
-        _require_cuda(name, t)
+    _all_tensors(qkv=qkv, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin, positions=positions,
+                 k_pool=k_pool, v_pool=v_pool, block_tables=block_tables)
+    if not (qkv.is_cuda and k_pool.is_cuda and v_pool.is_cuda and block_tables.is_cuda):
+        for name, t in (("k_pool", k_pool), ("v_pool", v_pool), ("block_tables", block_tables), ("qkv", qkv)):
+            _require_cuda(name, t)
     if k_pool.dim() != 4 or k_pool.shape != v_pool.shape or k_pool.dtype != v_pool.dtype:
         raise ValueError("k_pool and v_pool must be [num_blocks, H, block_size, D] of one dtype")
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("the pools must be contiguous")
     num_blocks, kv_heads, block_size, pool_dim = k_pool.shape
-    _require_cuda("qkv", qkv)
     if pool_dim == 0 or qkv.dim() < 1 or qkv.shape[-1] % pool_dim or \
             qkv.shape[-1] // pool_dim <= 2 * kv_heads:
         raise ValueError(f"qkv's last dimension does not hold queries beside {kv_heads} keys and "
@@ -1039,7 +1066,10 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
     if sid is None and bt.shape[0] != n:
         raise ValueError(f"without seq_ids there is one token per sequence: {n} tokens, "
                          f"{bt.shape[0]} sequences")
-    q = _out_tensor("out", out, lead + (heads, dim), qkv.dtype, device)
+    if out is None:
+        q = qkv.new_empty(lead + (heads, dim))
+    else:
+        q = _out_tensor("out", out, lead + (heads, dim), qkv.dtype, device)
     kp, vp = k_pool.data_ptr(), v_pool.data_ptr()
     pool_bytes = k_pool.numel() * k_pool.element_size()
     if kp < vp + pool_bytes and vp < kp + pool_bytes and pool_bytes:
@@ -1072,9 +1102,11 @@ def qk_norm_rope_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, qkv: torch
     without it), the weights' gradients are fp32, summed over tokens and heads in an order
     that depends on the sizes alone.
     """
-    _require_cuda("grad_q", grad_q)
-    _require_cuda("grad_k", grad_k)
-    _require_cuda("qkv", qkv)
+    _all_tensors(grad_q=grad_q, grad_k=grad_k, qkv=qkv, q_weight=q_weight, k_weight=k_weight,
+                 cos_sin=cos_sin, positions=positions)
+    if not (grad_q.is_cuda and grad_k.is_cuda and qkv.is_cuda):
+        for name, t in (("grad_q", grad_q), ("grad_k", grad_k), ("qkv", qkv)):
+            _require_cuda(name, t)
     if grad_q.dim() < 2 or grad_k.dim() < 2:
         raise ValueError("grad_q and grad_k must be [..., heads, head_dim]")
     heads, kv_heads = grad_q.shape[-2], grad_k.shape[-2]
@@ -1084,13 +1116,14 @@ def qk_norm_rope_backward(grad_q: torch.Tensor, grad_k: torch.Tensor, qkv: torch
     gq = _aligned(_same("grad_q", grad_q, lead + (heads, dim), qkv.dtype, device))
     gk = _aligned(_same("grad_k", grad_k, lead + (kv_heads, dim), qkv.dtype, device))
     gv = None if grad_v is None else _aligned(_same("grad_v", grad_v, lead + (kv_heads, dim), qkv.dtype, device))
-    grad = _out_tensor("out", out, tuple(qkv.shape), qkv.dtype, device)
-    if out is not None:
+    if out is None:
+        grad = qkv.new_empty(qkv.shape)
+    else:
+        grad = _out_tensor("out", out, tuple(qkv.shape), qkv.dtype, device)
         _apart("out", grad, qkv=rows, grad_q=gq, grad_k=gk, grad_v=gv)
     nbytes = _cached_bytes(lib.tome_qk_norm_rope_backward_workspace_bytes, dim)
     ws = _workspace(nbytes, device, workspace)
-    dqw = torch.empty(dim, dtype=torch.float32, device=device)
-    dkw = torch.empty(dim, dtype=torch.float32, device=device)
+    dqw, dkw = cs.new_empty(dim), cs.new_empty(dim)
     with _on(device):
         status = lib.tome_qk_norm_rope_backward(
             gq.data_ptr(), gk.data_ptr(), _ptr(gv), rows.data_ptr(), code, n, heads, kv_heads, dim,
@@ -1139,8 +1172,10 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     ``workspace`` may name a scratch tensor of :func:`shared_prefix_attention_workspace_bytes` bytes,
     which a decode loop reuses from step to step; calls that overlap in time need one each.
     """
-    for name, t in (("q", q), ("k_pool", k_pool), ("v_pool", v_pool)):
-        _require_cuda(name, t)
+    _all_tensors(q=q, k_pool=k_pool, v_pool=v_pool)
+    if not (q.is_cuda and k_pool.is_cuda and v_pool.is_cuda):
+        for name, t in (("q", q), ("k_pool", k_pool), ("v_pool", v_pool)):
+            _require_cuda(name, t)
     if q.dtype not in (torch.bfloat16, torch.float16):
         raise TypeError(f"q must be bfloat16 or float16, got {q.dtype}")
     if q.dim() != 3:
@@ -1155,7 +1190,9 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
     if not (k_pool.is_contiguous() and v_pool.is_contiguous()):
         raise ValueError("the pools must be contiguous")
     num_blocks, kv_heads, block_size, _ = k_pool.shape
-    if q.stride(2) == 1 and q.stride(1) == dim and (q.stride(0) >= heads * dim or n <= 1) and \
+    if q.is_contiguous() and q.data_ptr() % 16 == 0:
+        q_stride = heads * dim
+    elif q.stride(2) == 1 and q.stride(1) == dim and (q.stride(0) >= heads * dim or n <= 1) and \
             q.stride(0) % 8 == 0 and q.data_ptr() % 16 == 0:
         q_stride = q.stride(0) if n > 1 else heads * dim
     else:
@@ -1177,8 +1214,10 @@ def shared_prefix_attention(q: torch.Tensor, k_pool: torch.Tensor, v_pool: torch
         pt = _ints("prefix_tables", prefix_tables, prefix_tables.shape, device)
         plen = _ints("prefix_lens", prefix_lens, (groups,), device)
         starts = _ints("group_starts", group_starts, (groups + 1,), device)
-    o = _out_tensor("out", out, (n, heads, dim), q.dtype, device)
-    if out is not None:
+    if out is None:
+        o = q.new_empty((n, heads, dim))
+    else:
+        o = _out_tensor("out", out, (n, heads, dim), q.dtype, device)
         _apart("out", o, q=q, k_pool=k_pool, v_pool=v_pool)
     if out_lse is not None:
         _out_tensor("out_lse", out_lse, (n, heads), torch.float32, device)
@@ -1207,8 +1246,7 @@ def grpo_policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logprobs: torc
                      ref_logprobs: Optional[torch.Tensor] = None, clip_low: float = 0.2,
                      clip_high: float = 0.2, kl_coef: float = 0.0, reduction: str = "token",
                      grad_scale: float = 1.0, return_grad: bool = True, check: bool = False,
-                     out_grad: Optional[torch.Tensor] = None,
-                     workspace: Optional[torch.Tensor] = None):
+                     out_grad: Optional[torch.Tensor] = None):
     """Clipped policy loss with a k3 KL term and its gradient with respect to the logits.
 
     ``logits`` is ``[n_seq, seq_len, V]`` (bf16 or fp32); ``ids``, ``old_logprobs`` (the rollout's) and
@@ -1229,7 +1267,8 @@ def grpo_policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logprobs: torc
     logits.  The logits are read from HBM once and the gradient is written once; rows outside
     the windows are not read.  ``temp`` of 0 or None means 1.0.
     """
-    _require_cuda("logits", logits)
+    if not isinstance(logits, torch.Tensor) or not logits.is_cuda:
+        _require_cuda("logits", logits)
     if logits.dtype not in _DTYPES:
         _dtype_code(logits)
     if logits.dim() != 3:
@@ -1243,12 +1282,15 @@ def grpo_policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logprobs: torc
     temp = float(temp or 1.0)
     n_seq, seq_len, V = logits.shape
     device = logits.device
-    lg = _aligned(logits.detach())
+    lg = _aligned(logits.detach() if logits.requires_grad else logits)
     ids32 = _index(ids, n_seq * seq_len, device)
     len32 = _index(lengths, n_seq, device)
     st32 = None if starts is None else _index(starts, n_seq, device)
 
     def floats(name, t):
+        if isinstance(t, torch.Tensor) and t.dtype is torch.float32 and t.device == device and \
+                t.is_contiguous():
+            return t
         if not isinstance(t, torch.Tensor) or not t.is_floating_point():
             raise TypeError(f"{name} must be a floating-point tensor")
         if t.device != device:
@@ -1259,26 +1301,24 @@ def grpo_policy_loss(logits: torch.Tensor, ids: torch.Tensor, old_logprobs: torc
     adv = floats("advantages", advantages)
     ref = floats("ref_logprobs", ref_logprobs) if kl_coef else None
     for name, t in (("old_logprobs", old), ("ref_logprobs", ref)):
-        if t is not None and tuple(t.shape) != (n_seq, seq_len):
+        if t is not None and t.shape != (n_seq, seq_len):
             raise ValueError(f"{name} must be [n_seq, seq_len] = {(n_seq, seq_len)}, got {tuple(t.shape)}")
-    if tuple(adv.shape) not in ((n_seq,), (n_seq, seq_len)):
+    if adv.shape != (n_seq,) and adv.shape != (n_seq, seq_len):
         raise ValueError(f"advantages must be [n_seq] or [n_seq, seq_len], got {tuple(adv.shape)}")
     grad = None
     if return_grad:
-        grad = _out_tensor("out_grad", out_grad, (n_seq, seq_len, V), logits.dtype, device)
-        if out_grad is not None:
+        if out_grad is None:
+            grad = lg.new_empty((n_seq, seq_len, V))
+        else:
+            grad = _out_tensor("out_grad", out_grad, (n_seq, seq_len, V), logits.dtype, device)
             _apart("out_grad", grad, logits=lg)
-    loss = torch.empty((), dtype=torch.float32, device=device)
-    lp = torch.empty((n_seq, seq_len), dtype=torch.float32, device=device)
-    nbytes = _cached_bytes(lib.tome_grpo_policy_loss_workspace_bytes, n_seq, seq_len)
-    ws = _workspace(nbytes, device, workspace)
+    loss, lp = old.new_empty(()), old.new_empty((n_seq, seq_len))
     with _on(device):
         status = lib.tome_grpo_policy_loss(
             lg.data_ptr(), _DTYPES[lg.dtype], n_seq, seq_len, V, ids32.data_ptr(), old.data_ptr(), _ptr(ref),
             adv.data_ptr(), int(adv.dim() == 2), len32.data_ptr(), _ptr(st32), temp, float(clip_low),
             float(clip_high), float(kl_coef), int(reduction == "sequence"), float(grad_scale),
-            loss.data_ptr(), lp.data_ptr(), _ptr(grad), ws.data_ptr(), ws.numel() * ws.element_size(),
-            _status_word(device).data_ptr(), _stream(device))
+            loss.data_ptr(), lp.data_ptr(), _ptr(grad), _status_word(device).data_ptr(), _stream(device))
     _lib.check(status)
     if check:
         check_device_status(device)
