@@ -231,3 +231,12 @@ def test_gradient_continues_through_autograd(cuda_device):
     (-((lp - old).exp() * adv[:, None]) * mask).sum().div(5).backward()
     # two fp32 products of 16 and 6 terms, and the loss's own fp32 gradient
     assert float((got - w.grad).abs().max()) <= 2.0 ** -14 * float(w.grad.abs().max())
+
+
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 2500])
+def test_many_sequences(cuda_device, n):
+    """Many short sequences, most of them with rows outside their windows."""
+    c = _case(n, 3, 300, torch.bfloat16, 13)
+    starts = torch.randint(0, 4, (n,), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
+    _run(c, cuda_device, starts)
+    _run(c, cuda_device, None, reduction="sequence", return_grad=False)
