@@ -290,3 +290,17 @@ def test_random_shapes(cuda_device):
         prefix = torch.randint(0, pick([2, 100, 3000]), (len(sizes),), generator=g).tolist()
         _run(_case(100 + i, sizes, lens, prefix, pick([4, 16, 17, 64]), heads, kv, pick([64, 128]),
                    pick([torch.bfloat16, torch.float16])), cuda_device)
+
+
+@pytest.mark.parametrize("seed", range(40, 64))
+def test_more_random_batches(cuda_device, seed):
+    """Groups from one to many sequences, prompts and completions from nothing to several tiles."""
+    g = torch.Generator().manual_seed(seed)
+    pick = lambda *x: x[int(torch.randint(0, len(x), (1,), generator=g))]  # noqa: E731
+    groups = [int(x) for x in torch.randint(0, pick(2, 9, 20), (pick(1, 3, 6),), generator=g)]
+    n = max(1, sum(groups) + pick(0, 2))
+    lengths = [int(x) for x in torch.randint(0, pick(2, 40, 300), (n,), generator=g)]
+    prefix = [int(x) for x in torch.randint(0, pick(2, 100, 900), (len(groups),), generator=g)]
+    kv = pick(1, 2, 5)
+    _run(_case(seed, groups, lengths, prefix, pick(8, 13, 16, 32), kv * pick(1, 2, 4, 7, 8), kv, pick(64, 128),
+               pick(torch.bfloat16, torch.float16)), cuda_device)
