@@ -258,3 +258,19 @@ def test_side_stream_and_captured_graph(cuda_device):
     want = tome_b200.qk_norm_rope(qkv, qw, kw, table, pos, heads, kv)
     want_g = tome_b200.qk_norm_rope_backward(dq, dk, qkv, qw, kw, table, pos)
     assert all(torch.equal(a, b) for a, b in zip(want + want_g, got + got_g))
+
+
+@pytest.mark.parametrize("tokens,heads,kv,dim", [(1, 1, 1, 64), (400, 3, 1, 64), (401, 5, 3, 48), (333, 3, 3, 128)])
+def test_backward_without_eps(cuda_device, tokens, heads, kv, dim):
+    """Odd heads and tokens: what a group of threads does not have adds nothing to the weights' sums."""
+    import tome_b200
+    qkv, qw, kw, table, pos, g = _inputs(tokens, heads, kv, dim, torch.float32, tokens)
+    dq, dk = (torch.randn((tokens, n, dim), generator=g) for n in (heads, kv))
+    got = tome_b200.qk_norm_rope_backward(*(x.to(cuda_device) for x in (dq, dk, qkv, qw, kw, table, pos)), eps=0.0, check=True)
+    x, dx = qkv.view(tokens, heads + 2 * kv, dim), got[0].view(tokens, heads + 2 * kv, dim)
+    for part, w, d, at, gw in ((x[:, :heads], qw, dq, dx[:, :heads], got[1]),
+                               (x[:, heads:heads + kv], kw, dk, dx[:, heads:heads + kv], got[2])):
+        want, dw, size, wsize = step.norm_rope_backward(part, w, d, table, pos, 0.0)
+        _close(at, want, size, torch.float32)
+        chain = 64 + 50 + tokens * heads // 64
+        assert bool(((gw.cpu().double() - dw).abs() <= chain * F32 * wsize + 1e-30).all())

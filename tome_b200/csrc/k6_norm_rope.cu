@@ -373,7 +373,8 @@ __global__ void __launch_bounds__(K6_THREADS, sizeof(T) == 4 ? 1 : K6_B_MINB) k6
       for (int i = 0; i < HPG; ++i) {
         const K6Eight a = k6_unpack(xl[i]), b = k6_unpack(xh[i]);
         const float ss = k6_group_sum<G>(k6_squares(a, b));
-        float r = rsqrtf(fmaf(ss, inv_dim, p.eps));
+        // 0 for a head that is not there: with an eps of 0 its zeros would become NaN in the sums
+        float r = i < n ? rsqrtf(fmaf(ss, inv_dim, p.eps)) : 0.0f;
         if (bad) r = __int_as_float(0x7fc00000);
         const K6Eight da = k6_unpack(gl[i]), db = k6_unpack(gh[i]), wa = k6_unpack(w_lo), wb = k6_unpack(w_hi);
         K6Eight ya, yb;  // gradient of the normed head (rotation turned back), times the weight
