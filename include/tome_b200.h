@@ -359,7 +359,7 @@ int32_t tome_qk_norm_rope(const void* qkv, int32_t dtype, int64_t tokens, int32_
  * Unlike tome_update_paged_kv it writes anywhere in a block, so a decode step appends one token.
  * cache_positions[t] < 0: the token is not cached.  A place that the table or the pool does not
  * have is skipped and sets TOME_DEV_BLOCK_OUT_OF_RANGE; a token whose position is bad gets NaN
- * queries and no key.  Two tokens of a call that name one place race.
+ * queries and is not cached.  Two tokens of a call that name one place race.
  */
 int32_t tome_qk_norm_rope_append(const void* qkv, int32_t dtype, int64_t tokens, int32_t heads,
                                  int32_t kv_heads, int32_t head_dim, int64_t qkv_stride,

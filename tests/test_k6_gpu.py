@@ -274,3 +274,24 @@ def test_backward_without_eps(cuda_device, tokens, heads, kv, dim):
         _close(at, want, size, torch.float32)
         chain = 64 + 50 + tokens * heads // 64
         assert bool(((gw.cpu().double() - dw).abs() <= chain * F32 * wsize + 1e-30).all())
+
+
+def test_append_of_bad_positions_leaves_the_place_as_it_was(cuda_device):
+    """Neither the key nor the value is cached: a place never holds a key of one token and a value of another."""
+    import tome_b200
+    heads, kv, dim, block, n = 2, 2, 64, 4, 5
+    qkv, qw, kw, table, pos, g = _inputs(n, heads, kv, dim, torch.bfloat16, 9)
+    pos[1], pos[3] = -1, table.shape[0]
+    pool = torch.randn((n, kv, block, dim), generator=g).to(torch.bfloat16).to(cuda_device)
+    kp, vp = pool.clone(), pool.clone()
+    tables = torch.arange(n, dtype=torch.int32, device=cuda_device)[:, None].contiguous()
+    at = torch.full((n,), 2, dtype=torch.int32, device=cuda_device)
+    q = tome_b200.qk_norm_rope_append(*(x.to(cuda_device) for x in (qkv, qw, kw, table, pos)), kp, vp, tables, at)
+    with pytest.raises(tome_b200.TomeRuntimeError, match="rotary"):
+        tome_b200.check_device_status(cuda_device)
+    assert q.isnan().flatten(1).all(1).tolist() == [False, True, False, True, False]
+    for t in range(n):
+        changed = t not in (1, 3)
+        for p in (kp, vp):
+            assert bool((p[t, :, 2] != pool[t, :, 2]).any()) == changed
+            assert torch.equal(p[t, :, [0, 1, 3]], pool[t, :, [0, 1, 3]])

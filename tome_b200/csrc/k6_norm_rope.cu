@@ -239,8 +239,9 @@ __global__ void __launch_bounds__(K6_THREADS, HPG == 1 ? 3 : (sizeof(T) == 4 ? 1
       } else if (p.k_out != nullptr) {
         dst = reinterpret_cast<T*>(p.k_out) + (t * p.kv_heads + h0) * p.dim + j * 8;
       } else {
-        const int32_t at = p.cache_pos[t];
-        if (at >= 0) {
+        const int32_t at = p.cache_pos[t], pos = p.positions[t];
+        // a token whose rotary position is bad (its keys report it) is not cached at all
+        if (at >= 0 && pos >= 0 && pos < p.n_positions) {
           const int64_t seq = p.seq_ids != nullptr ? static_cast<int64_t>(p.seq_ids[t]) : t;
           const int32_t blk = at / p.block_size;
           int32_t page = -1;
@@ -297,8 +298,7 @@ __global__ void __launch_bounds__(K6_THREADS, HPG == 1 ? 3 : (sizeof(T) == 4 ? 1
         za.v[e] = __ffma2_rn(ya, co.v[e], __fmul2_rn(k6_neg(yb), si.v[e]));
         zb.v[e] = __ffma2_rn(yb, co.v[e], __fmul2_rn(ya, si.v[e]));
       }
-      // a key whose position is bad is not cached
-      if (i < n && kind != 2 && dst != nullptr && !(bad && kind == 1 && p.k_out == nullptr)) {
+      if (i < n && kind != 2 && dst != nullptr) {
         k6_store(dst + i * pitch, k6_pack8<T>(za));
         k6_store(dst + i * pitch + half, k6_pack8<T>(zb));
       }

@@ -1035,8 +1035,9 @@ def qk_norm_rope_append(qkv: torch.Tensor, q_weight: torch.Tensor, k_weight: tor
     :func:`update_paged_kv`, which writes whole blocks from their start, it writes anywhere in
     a block.  ``positions`` are the rotary positions, which differ from the places where a
     shared prefix has pages of its own (:func:`shared_prefix_attention`).  A place that the table
-    or the pool does not have is skipped and reported through the device status; two tokens of
-    a call must not name the same place.
+    or the pool does not have is skipped and reported through the device status, and so is a token whose
+    rotary position the table ``cos_sin`` does not have (its queries are NaN); two tokens of a call must
+    not name the same place.
     """
     _all_tensors(qkv=qkv, q_weight=q_weight, k_weight=k_weight, cos_sin=cos_sin, positions=positions,
                  k_pool=k_pool, v_pool=v_pool, block_tables=block_tables)
