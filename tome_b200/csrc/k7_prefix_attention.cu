@@ -542,12 +542,18 @@ __device__ __forceinline__ void k7_mma(float (&c)[4], const uint32_t (&a)[4], ui
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 
+// A whole warp waits.  Either all its lanes go on or none does: one lane whose wait ran out must not
+// leave the others at a vote.
+__device__ __forceinline__ bool k7_wait(uint32_t bar, uint32_t parity) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, parity));
+}
+
 // All softmax warps meet: what each wrote before is visible to all behind.  An mbarrier rather than
 // a hardware barrier, so that the wait has a limit too; `met` counts the meetings.
 __device__ __forceinline__ void k7_meet(const K7Params& p, uint32_t bar, uint32_t& met, int lane, bool& ok) {
   __syncwarp();
   if (lane == 0) mbar_arrive(bar);
-  if (ok && !mbar_wait(bar, met & 1u)) {
+  if (ok && !k7_wait(bar, met & 1u)) {
     k7_raise(p.status, TOME_DEV_TIMEOUT);
     ok = false;
   }
@@ -670,11 +676,8 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const CUtensorMa
       __syncwarp();  // the tile before, whose place is filled now, is done with
       fill();
       const uint32_t read_at = (used % K7_SMALL_STAGES) * S::SMALL_STAGE;
-      if (!mbar_wait(full + (used % K7_SMALL_STAGES) * 8, (used / K7_SMALL_STAGES) & 1u)) {
-        k7_raise(p.status, TOME_DEV_TIMEOUT);
-        asm volatile("cp.async.wait_all;" ::: "memory");
-        return;
-      }
+      // (whether it came is voted on below, together with the maxima: a vote of its own took another 1.5 %)
+      const bool there = mbar_wait(full + (used % K7_SMALL_STAGES) * 8, (used / K7_SMALL_STAGES) & 1u);
       __syncwarp();
       ++used;
       float s[2][4] = {}, s2[2][4] = {};  // two chains of products for each eight keys
@@ -706,13 +709,18 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const CUtensorMa
       // The exponents' reference moves only when a score exceeds it by more than 2^8, which one
       // vote finds out; the row maxima are formed only then.
       float top[2];
-      bool grow = false;
+      bool grow = !there;
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
         top[r] = fmaxf(fmaxf(s[0][2 * r], s[0][2 * r + 1]), fmaxf(s[1][2 * r], s[1][2 * r + 1])) * p.c;
         grow |= top[r] > ref[r] + 8.0f;
       }
       if (__any_sync(0xffffffffu, grow)) {
+        if (!__all_sync(0xffffffffu, there)) {  // the whole warp gives up
+          k7_raise(p.status, TOME_DEV_TIMEOUT);
+          asm volatile("cp.async.wait_all;" ::: "memory");
+          return;
+        }
 #pragma unroll
         for (int r = 0; r < 2; ++r) {
           top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
@@ -793,12 +801,11 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
   const uint32_t end = u + x.n, mine = u + ((u ^ team) & 1u);
   for (uint32_t i = mine; i < end && ok; i += 2) {
     // S of this tile, and P V of the team's tile before: P may be written, the sums be rescaled
-    if (!mbar_wait(base + S::S_FULL + team * 8, (i >> 1) & 1u) ||
-        (i > mine && !mbar_wait(base + S::O_FULL + team * 8, ((i >> 1) - 1) & 1u))) {
+    if (!k7_wait(base + S::S_FULL + team * 8, (i >> 1) & 1u) ||
+        (i > mine && !k7_wait(base + S::O_FULL + team * 8, ((i >> 1) - 1) & 1u))) {
       k7_raise(p.status, TOME_DEV_TIMEOUT);
       ok = false;
     }
-    __syncwarp();
     if (active) {
       tc_fence_after_sync();
       uint32_t s0[32], s1[32];
@@ -867,11 +874,10 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
   float2* const ml = reinterpret_cast<float2*>(smem + S::MEET_ML);
   if (mine < end && ok) {
     const uint32_t i = end - 1 - ((end - 1 - mine) & 1u);  // the team's last tile
-    if (!mbar_wait(base + S::O_FULL + team * 8, (i >> 1) & 1u)) {
+    if (!k7_wait(base + S::O_FULL + team * 8, (i >> 1) & 1u)) {
       k7_raise(p.status, TOME_DEV_TIMEOUT);
       ok = false;
     }
-    __syncwarp();
     tc_fence_after_sync();
   }
   u = end;
@@ -978,7 +984,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
       // ---------------------------------------------------------- softmax
       uint32_t u = 0, piece = 0, met = 0;  // tiles, pieces, meetings so far; a tile's team is its parity
       for (bool ok = true; ok; ++piece) {
-        if (!mbar_wait(base + S::CARD_FULL + (piece % K7_CARDS) * 8, (piece / K7_CARDS) & 1u)) {
+        if (!k7_wait(base + S::CARD_FULL + (piece % K7_CARDS) * 8, (piece / K7_CARDS) & 1u)) {
           k7_raise(p.status, TOME_DEV_TIMEOUT);
           break;
         }
@@ -1043,7 +1049,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
           u = end;
         }
         // nothing may still be under way when the space is used otherwise
-        if (ok && any && !mbar_wait(base + S::O_FULL + team * 8, (last_mine >> 1) & 1u)) ok = false;
+        if (any && !mbar_wait(base + S::O_FULL + team * 8, (last_mine >> 1) & 1u)) ok = false;
         if (!ok) k7_raise(p.status, TOME_DEV_TIMEOUT);
       }
       __syncwarp();
@@ -1084,7 +1090,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
             show(next, piece + 1, next_there);
             if (next_there) next_pages = k7_open_pages(p, next, next.tile * K7_KEYS, lane);
           }
-          if (t >= stages && !mbar_wait(empty + stage * 8, (t / stages - 1) & 1u)) {
+          if (t >= stages && !k7_wait(empty + stage * 8, (t / stages - 1) & 1u)) {
             k7_raise(p.status, TOME_DEV_TIMEOUT);
             ok = false;
             break;
