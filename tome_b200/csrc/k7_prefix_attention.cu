@@ -75,6 +75,7 @@ struct K7Params {
   int32_t div_shift, ratio_shift;
   float c;                    // scale * log2(e)
   bool whole_pages;           // pages of a multiple of 16 tokens: tiles go by tensor copies
+  int32_t big_box;            // sixteens of rows per tensor copy of a big tile: 1, 2 or 4
   int32_t ctas;               // CTAs of the main kernel
   double inv_ctas;            // 1 / ctas
   // workspace: the pieces' rows, those of big prefix items (128 per piece), of small ones (16) from
@@ -429,10 +430,11 @@ struct K7Card {
 // at r * 128 + ((c ^ (r & 7)) << 4).
 template <int D>
 struct K7Smem {
-  // tensor memory: S 2 x 64 columns, O 2 x D, P 2 x 32 (two 16-bit values per column)
-  static constexpr int O_COL = 2 * K7_KEYS;
-  static constexpr int P_COL = O_COL + 2 * D;
+  // tensor memory: each team's two S (64 columns; P, two 16-bit values per column, takes the place of
+  // the S it is made of), then each team's O
+  static constexpr int O_COL = 4 * K7_KEYS;
   static constexpr int TMEM_COLS = 512;
+  static_assert(O_COL + 2 * D <= TMEM_COLS, "tensor memory");
   static constexpr int Q_BYTES = K7_ROWS * D * 2;
   static constexpr int KV_BYTES = K7_KEYS * D * 2;
   static constexpr int Q = 0;
@@ -449,9 +451,9 @@ struct K7Smem {
   static constexpr int K_EMPTY = K_FULL + K7_K_STAGES * 8;
   static constexpr int V_FULL = K_EMPTY + K7_K_STAGES * 8;
   static constexpr int V_EMPTY = V_FULL + K7_V_STAGES * 8;
-  static constexpr int S_FULL = V_EMPTY + K7_V_STAGES * 8; // 2 (teams), as the next three
-  static constexpr int P_FULL = S_FULL + 16;
-  static constexpr int O_FULL = P_FULL + 16;
+  static constexpr int S_FULL = V_EMPTY + K7_V_STAGES * 8; // 2 (teams) x 2, as the next
+  static constexpr int P_FULL = S_FULL + 32;
+  static constexpr int O_FULL = P_FULL + 32;               // 2 (teams), as the next
   static constexpr int Q_FULL = O_FULL + 16;
   static constexpr int MEET = Q_FULL + 16;                 // the softmax warps among themselves
   static constexpr int TMEM = MEET + 16;
@@ -800,17 +802,17 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
   float ref = -INFINITY, sum = 0.0f;
   const uint32_t end = u + x.n, mine = u + ((u ^ team) & 1u);
   for (uint32_t i = mine; i < end && ok; i += 2) {
-    // S of this tile, and P V of the team's tile before: P may be written, the sums be rescaled
-    if (!k7_wait(base + S::S_FULL + team * 8, (i >> 1) & 1u) ||
-        (i > mine && !k7_wait(base + S::O_FULL + team * 8, ((i >> 1) - 1) & 1u))) {
+    const uint32_t n = i >> 1, half = 2 * team + (n & 1u);  // the team's n-th tile, in its S number n & 1
+    const uint32_t s_addr = tmem + lanes + half * K7_KEYS;
+    if (!k7_wait(base + S::S_FULL + half * 8, (n >> 1) & 1u)) {
       k7_raise(p.status, TOME_DEV_TIMEOUT);
       ok = false;
     }
     if (active) {
       tc_fence_after_sync();
       uint32_t s0[32], s1[32];
-      tmem_ld32(tmem + lanes + team * K7_KEYS, s0);
-      tmem_ld32(tmem + lanes + team * K7_KEYS + 32, s1);
+      tmem_ld32(s_addr, s0);
+      tmem_ld32(s_addr + 32, s1);
       tmem_ld_wait_dep(s0);
       tmem_ld_wait_dep(s1);
       const int32_t valid = x.len - (x.tile + static_cast<int32_t>(i - u)) * K7_KEYS;
@@ -834,6 +836,12 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
         sum *= alpha;
         ref = next;
         if (i > mine) {
+          // P V of the team's tile before is done (the next one waits for this tile's P)
+          if (!k7_wait(base + S::O_FULL + team * 8, (n - 1) & 1u)) {
+            k7_raise(p.status, TOME_DEV_TIMEOUT);
+            ok = false;
+          }
+          tc_fence_after_sync();
 #pragma unroll 1
           for (int h = 0; h < D; h += 32) {
             uint32_t r[32];
@@ -861,20 +869,27 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
         else lb = __fadd2_rn(lb, e);
         pw[k] = k7_pack(e.x, e.y, T());
       }
-      tmem_st32(tmem + lanes + S::P_COL + team * (K7_KEYS / 2), pw);
+      tmem_st32(s_addr, pw);
       sum += (la.x + la.y) + (lb.x + lb.y);
       tmem_st_wait();
       tc_fence_before_sync();
     }
+    // The piece's last P is handed over when P V of the tile before is done: a phase is known by its
+    // parity alone, so that the wait for the last P V must not find the one before under way.  (The
+    // phase before that one is over, S of this tile was made behind it.)
+    if (i > mine && i + 2 >= end && !k7_wait(base + S::O_FULL + team * 8, (n - 1) & 1u)) {
+      k7_raise(p.status, TOME_DEV_TIMEOUT);
+      ok = false;
+    }
     __syncwarp();
-    if (lane == 0) mbar_arrive(base + S::P_FULL + team * 8);
+    if (lane == 0) mbar_arrive(base + S::P_FULL + half * 8);
   }
   // The teams' sums meet: each team brings the rows' reference and sum, then writes half of the
   // columns from both teams' O.
   float2* const ml = reinterpret_cast<float2*>(smem + S::MEET_ML);
   if (mine < end && ok) {
-    const uint32_t i = end - 1 - ((end - 1 - mine) & 1u);  // the team's last tile
-    if (!k7_wait(base + S::O_FULL + team * 8, (i >> 1) & 1u)) {
+    const uint32_t n = (end - 1 - ((end - 1 - mine) & 1u)) >> 1;  // the team's last tile
+    if (!k7_wait(base + S::O_FULL + team * 8, n & 1u)) {
       k7_raise(p.status, TOME_DEV_TIMEOUT);
       ok = false;
     }
@@ -926,7 +941,8 @@ __device__ __forceinline__ bool k7_big_piece(const K7Params& p, uint8_t* smem, u
 // 1700 clocks per tile.)
 template <typename T, int D>
 __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
-    const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map, const K7Params p) {
+    const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map,
+    const __grid_constant__ CUtensorMap k_map_16, const __grid_constant__ CUtensorMap v_map_16, const K7Params p) {
   using S = K7Smem<D>;
   extern __shared__ uint8_t smem_raw[];
   const uint32_t raw = smem_u32(smem_raw);
@@ -950,9 +966,11 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
       mbar_init(base + S::V_FULL + i * 8, 32);
       mbar_init(base + S::V_EMPTY + i * 8, 1);
     }
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < 4; ++i) {
       mbar_init(base + S::S_FULL + i * 8, 1);
       mbar_init(base + S::P_FULL + i * 8, K7_TEAM_WARPS);
+    }
+    for (int i = 0; i < 2; ++i) {
       mbar_init(base + S::O_FULL + i * 8, 1);
       mbar_init(base + S::Q_FULL + i * 8, K7_SOFTMAX_WARPS * 32);
     }
@@ -999,57 +1017,61 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
         const uint32_t team = warp == K7_ISSUE_WARP ? 0u : 1u;
         const uint64_t q_desc = k7_desc_k(base + S::Q), k_desc = k7_desc_k(base + S::K);
         const uint64_t v_desc = k7_desc_mn(base + S::V, K7_KEYS * 128);
-        const uint32_t s_addr = tmem + team * K7_KEYS, o_addr = tmem + S::O_COL + team * D;
-        const uint32_t p_addr = tmem + S::P_COL + team * (K7_KEYS / 2);
+        const uint32_t s_addr = tmem + 2 * team * K7_KEYS, o_addr = tmem + S::O_COL + team * D;
+        const uint32_t s_full = base + S::S_FULL + 16 * team, p_full = base + S::P_FULL + 16 * team;
+        const uint32_t o_full = base + S::O_FULL + 8 * team;
         uint32_t u = 0, piece = 0, pieces = 0, last_mine = 0;  // `pieces`: those with a tile of the team
         bool ok = true, any = false;
-        // P of the team's tile `i` is there, and its S is read
-        auto wait_p = [&](uint32_t i) {
-          if (!mbar_wait(base + S::P_FULL + team * 8, (i >> 1) & 1u)) ok = false;
+        auto multiply_qk = [&](uint32_t i) {  // S = Q K^T of tile i
+          const uint32_t stage = i % K7_K_STAGES, half = (i >> 1) & 1u;
+          if (!mbar_wait(base + S::K_FULL + stage * 8, (i / K7_K_STAGES) & 1u)) ok = false;
+          if (!ok) return;
+          fence_proxy_async();  // tiles that did not come by tensor copies are ordinary writes
+          tc_fence_after_sync();
+          const uint64_t a = q_desc, b = k_desc + stage * (S::KV_BYTES >> 4);
+#pragma unroll
+          for (int k = 0; k < D / 16; ++k)
+            umma_bf16_ss(s_addr + half * K7_KEYS, a + (k / 4) * (K7_ROWS * 128 >> 4) + 2 * (k % 4),
+                         b + (k / 4) * (K7_KEYS * 128 >> 4) + 2 * (k % 4), k7_idesc<T>(K7_KEYS, false), k != 0);
+          umma_commit(s_full + half * 8);
+          umma_commit(base + S::K_EMPTY + stage * 8);
         };
         auto multiply_pv = [&](uint32_t i, bool add) {  // O (+)= P V of tile i
-          const uint32_t stage = i % K7_V_STAGES;
+          const uint32_t stage = i % K7_V_STAGES, half = (i >> 1) & 1u;
+          if (!mbar_wait(p_full + half * 8, (i >> 2) & 1u)) ok = false;
           if (!mbar_wait(base + S::V_FULL + stage * 8, (i / K7_V_STAGES) & 1u)) ok = false;
-          fence_proxy_async();  // tiles that did not come by tensor copies are ordinary writes
+          if (!ok) return;
+          fence_proxy_async();
           tc_fence_after_sync();
           const uint64_t b = v_desc + stage * (S::KV_BYTES >> 4);
 #pragma unroll
           for (int k = 0; k < K7_KEYS / 16; ++k)  // 16 keys: 8 columns of P, 16 rows of V
-            umma_f16_ts(o_addr, p_addr + 8 * k, b + (2048 >> 4) * k, k7_idesc<T>(D, true), add || k != 0);
-          umma_commit(base + S::O_FULL + team * 8);
+            umma_f16_ts(o_addr, s_addr + half * K7_KEYS + 8 * k, b + (2048 >> 4) * k, k7_idesc<T>(D, true), add || k != 0);
+          umma_commit(o_full);
           umma_commit(base + S::V_EMPTY + stage * 8);
+          any = true;
+          last_mine = i;
         };
         K7Piece x;
         int32_t at = first;
         for (; ok && k7_next<true>(p, pl, x, piece > 0, at, last); ++piece) {
           const uint32_t end = u + x.n, mine = u + ((u ^ team) & 1u);
-          for (uint32_t i = mine; i < end && ok; i += 2) {
-            const uint32_t stage = i % K7_K_STAGES;
-            if (i == mine && !mbar_wait(base + S::Q_FULL + team * 8, pieces++ & 1u)) ok = false;
-            if (!mbar_wait(base + S::K_FULL + stage * 8, (i / K7_K_STAGES) & 1u)) ok = false;
-            if (i > mine) wait_p(i - 2);
-            if (!ok) break;
-            fence_proxy_async();
-            tc_fence_after_sync();
-            const uint64_t a = q_desc, b = k_desc + stage * (S::KV_BYTES >> 4);
-#pragma unroll
-            for (int k = 0; k < D / 16; ++k)
-              umma_bf16_ss(s_addr, a + (k / 4) * (K7_ROWS * 128 >> 4) + 2 * (k % 4),
-                           b + (k / 4) * (K7_KEYS * 128 >> 4) + 2 * (k % 4), k7_idesc<T>(K7_KEYS, false), k != 0);
-            umma_commit(base + S::S_FULL + team * 8);
-            umma_commit(base + S::K_EMPTY + stage * 8);
-            if (i > mine) multiply_pv(i - 2, i - 2 > mine);
-            last_mine = i;
+          if (mine < end) {
+            if (!mbar_wait(base + S::Q_FULL + team * 8, pieces++ & 1u)) ok = false;
+            if (ok) multiply_qk(mine);
+            if (ok && mine + 2 < end) multiply_qk(mine + 2);
           }
-          if (mine < end && ok) {  // the softmax warps wait for the last tile's O
-            any = true;
-            wait_p(last_mine);
-            if (ok) multiply_pv(last_mine, last_mine > mine);
+          for (uint32_t i = mine; i < end && ok; i += 2) {
+            multiply_pv(i, i > mine);
+            if (!ok || i + 4 >= end) continue;
+            // the S that the tile's P lay in is free once that has been read
+            if (!mbar_wait(o_full, (i >> 1) & 1u)) ok = false;
+            if (ok) multiply_qk(i + 4);
           }
           u = end;
         }
         // nothing may still be under way when the space is used otherwise
-        if (any && !mbar_wait(base + S::O_FULL + team * 8, (last_mine >> 1) & 1u)) ok = false;
+        if (any && !mbar_wait(o_full, (last_mine >> 1) & 1u)) ok = false;
         if (!ok) k7_raise(p.status, TOME_DEV_TIMEOUT);
       }
       __syncwarp();
@@ -1120,10 +1142,12 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
             if (lane == 0) {
               mbar_expect_tx(full + stage * 8, S::KV_BYTES);
 #pragma unroll
-              for (int h = 0; h < K7_KEYS / 16; ++h)
+              for (int h = 0; h < K7_KEYS / 16; ++h) {
+                if (h & (p.big_box - 1)) continue;
 #pragma unroll
                 for (int b = 0; b < D / 64; ++b)
                   tma_load_2d(dst + b * (K7_KEYS * 128) + h * 2048, map, b * 64, rows[h], full + stage * 8);
+              }
             }
           } else {
             by_hand |= 1u << stage;
@@ -1191,7 +1215,7 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
   // the first workers are spread over the CTAs
   const int32_t worker = warp * gridDim.x + blockIdx.x;
   if (worker < small.workers)
-    k7_small_run<T, D>(p, &k_map, &v_map, pl, base + warp * (K7_SMALL_STAGES * S::SMALL_STAGE),
+    k7_small_run<T, D>(p, &k_map_16, &v_map_16, pl, base + warp * (K7_SMALL_STAGES * S::SMALL_STAGE),
                        base + S::SMALL_FULL + warp * (K7_SMALL_STAGES * 8), worker, small.begin(worker),
                        small.begin(worker + 1), lane);
 }
@@ -1329,19 +1353,24 @@ static int32_t k7_shape(int64_t n_seq, int64_t n_groups, int64_t heads, int64_t 
 template <typename T, int D>
 static int32_t k7_launch(const K7Params& p, cudaStream_t stream) {
   using S = K7Smem<D>;
-  void (*kernel)(CUtensorMap, CUtensorMap, K7Params) = k7_attention_kernel<T, D>;
+  void (*kernel)(CUtensorMap, CUtensorMap, CUtensorMap, CUtensorMap, K7Params) = k7_attention_kernel<T, D>;
   const int bytes = S::PLAN + S::plan_bytes(p.n_groups, p.n_seq) + 1024;
   // set once for the largest plan, so that no later call has to raise it
   const int most = S::PLAN + S::plan_bytes(K7_MAX_GROUPS, K7_MAX_SEQ) + 1024;
   static_assert(S::PLAN + S::plan_bytes(K7_MAX_GROUPS, K7_MAX_SEQ) + 1024 <= 232448, "shared memory");
   int32_t st = ensure_dynamic_smem(reinterpret_cast<const void*>(kernel), most);
   if (st != TOME_OK) return st;
-  // the pools as matrices of 64-column blocks, sixteen rows at a time
-  CUtensorMap k_map = {}, v_map = {};
+  // the pools as matrices of 64-column blocks, for small tiles sixteen rows at a time, for big ones as
+  // many as divide a page
+  CUtensorMap k_map = {}, v_map = {}, k_map_16 = {}, v_map_16 = {};
   if (p.whole_pages) {
     const int64_t rows = static_cast<int64_t>(p.num_blocks) * p.kv_heads * p.block_size;
-    st = tensor_map_16bit(&k_map, p.k_pool, rows, D, 16);
-    if (st == TOME_OK) st = tensor_map_16bit(&v_map, p.v_pool, rows, D, 16);
+    st = tensor_map_16bit(&k_map_16, p.k_pool, rows, D, 16);
+    if (st == TOME_OK) st = tensor_map_16bit(&v_map_16, p.v_pool, rows, D, 16);
+    k_map = k_map_16;
+    v_map = v_map_16;
+    if (p.big_box > 1 && st == TOME_OK) st = tensor_map_16bit(&k_map, p.k_pool, rows, D, 16 * p.big_box);
+    if (p.big_box > 1 && st == TOME_OK) st = tensor_map_16bit(&v_map, p.v_pool, rows, D, 16 * p.big_box);
     if (st != TOME_OK) return st;
   }
   cudaLaunchAttribute attr;  // each kernel is set up while the one before it drains
@@ -1354,7 +1383,7 @@ static int32_t k7_launch(const K7Params& p, cudaStream_t stream) {
   cfg.stream = stream;
   cfg.attrs = &attr;
   cfg.numAttrs = 1;
-  st = check_cuda(cudaLaunchKernelEx(&cfg, kernel, k_map, v_map, p), "prefix attention launch");
+  st = check_cuda(cudaLaunchKernelEx(&cfg, kernel, k_map, v_map, k_map_16, v_map_16, p), "prefix attention launch");
   if (st != TOME_OK) return st;
   // Few rows have many pieces each: a block of warps per row then, else a warp.
   const int64_t rows = static_cast<int64_t>(p.n_seq) * p.heads;
@@ -1449,6 +1478,7 @@ extern "C" int32_t tome_shared_prefix_attention(
   divisor(p.ratio, &p.ratio_magic, &p.ratio_shift);
   p.c = scale * LOG2E;
   p.whole_pages = block_size % 16 == 0 && num_blocks > 0;
+  p.big_box = block_size % 64 == 0 ? 4 : (block_size % 32 == 0 ? 2 : 1);
   p.ctas = std::max(1, std::min(info.sm_count, K7_MAX_CTAS));
   p.inv_ctas = 1.0 / p.ctas;
   uint8_t* ws = static_cast<uint8_t*>(workspace);
