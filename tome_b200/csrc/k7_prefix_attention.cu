@@ -610,14 +610,13 @@ __device__ __forceinline__ void k7_small_run(const K7Params& p, const CUtensorMa
           by_hand &= ~(1u << stage);
         }
         if (lane == 0) {
-          mbar_arrive_expect_tx(bar, S::SMALL_STAGE);
+          mbar_expect_tx(bar, S::SMALL_STAGE);
+          mbar_arrive_many(bar, 32);
 #pragma unroll
           for (int h = 0; h < D / 64; ++h) {
             tma_load_2d(dst + h * BLOCK, k_map, h * 64, row0, bar);
             tma_load_2d(dst + S::SMALL_KV + h * BLOCK, v_map, h * 64, row0, bar);
           }
-        } else {
-          mbar_arrive(bar);
         }
       } else {
         by_hand |= 1u << stage;
@@ -1098,19 +1097,43 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
       int32_t at = first;
       K7Piece x = {};
       K7Pages pages = {};
+      // Where whole pages hold them, the pool rows of a piece's groups of sixteen keys are looked up 32
+      // at a time, one per lane, and the pages behind those are asked for meanwhile: with a look-up per
+      // tile this warp, not the memory, set the pace.
+      auto page_of = [&](const K7Piece& y, int32_t group) {
+        const int32_t key = (group + lane) * 16;
+        return p.whole_pages && key + 16 <= y.len ? __ldg(y.table + k7_block(p, key)) : -1;
+      };
+      int32_t ahead = -1, row = -1;
+      uint32_t good = 0;  // the groups that have a row
       bool there = k7_next<true>(p, pl, x, false, at, last);
       show(x, 0, there);
-      if (there) pages = k7_open_pages(p, x, x.tile * K7_KEYS, lane);
+      if (there) {
+        pages = k7_open_pages(p, x, x.tile * K7_KEYS, lane);
+        ahead = page_of(x, x.tile * (K7_KEYS / 16));
+      }
       while (there && ok) {
         K7Piece next = x;
         K7Pages next_pages = {};
+        int32_t next_ahead = -1;
         bool next_there = false;
         for (int32_t j = 0; j < x.n; ++j, ++t) {
           const uint32_t stage = t % stages;
           if (j + 1 == x.n) {  // the piece behind is looked up while this one's loads are under way
             next_there = k7_next<true>(p, pl, next, true, at, last);
             show(next, piece + 1, next_there);
-            if (next_there) next_pages = k7_open_pages(p, next, next.tile * K7_KEYS, lane);
+            if (next_there) {
+              next_pages = k7_open_pages(p, next, next.tile * K7_KEYS, lane);
+              next_ahead = page_of(next, next.tile * (K7_KEYS / 16));
+            }
+          }
+          if (j % 8 == 0) {
+            const int32_t group = (x.tile + j) * (K7_KEYS / 16), key = (group + lane) * 16;
+            row = ahead < 0 || ahead >= p.num_blocks
+                      ? -1
+                      : (ahead * p.kv_heads + x.kv_head) * p.block_size + (key - k7_block(p, key) * p.block_size);
+            good = __ballot_sync(0xffffffffu, row >= 0);
+            if (j + 8 < x.n) ahead = page_of(x, group + 32);
           }
           if (t >= stages && !k7_wait(empty + stage * 8, (t / stages - 1) & 1u)) {
             k7_raise(p.status, TOME_DEV_TIMEOUT);
@@ -1120,16 +1143,8 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
           __syncwarp();
           const uint32_t dst = area + stage * S::KV_BYTES;
           const int32_t key0 = (x.tile + j) * K7_KEYS;
-          // pool rows of the tile's four groups of sixteen keys, one per lane, where whole pages hold them
-          const int32_t group = key0 + 16 * (lane & 3);
-          int32_t row = -1;
-          bool whole = p.whole_pages && key0 + K7_KEYS <= x.len;
-          if (whole) {
-            const int32_t blk = k7_block(p, group), page = k7_page(p, x, pages, k7_block(p, key0), blk, lane);
-            if (page >= 0 && page < p.num_blocks)
-              row = (page * p.kv_heads + x.kv_head) * p.block_size + (group - blk * p.block_size);
-            whole = __all_sync(0xffffffffu, row >= 0);
-          }
+          const int32_t in_batch = (j % 8) * (K7_KEYS / 16);
+          const bool whole = (good >> in_batch & 0xfu) == 0xfu;
           if (whole) {
             if (by_hand >> stage & 1u) {  // ordinary writes before the tensor copies'
               fence_proxy_async();
@@ -1138,9 +1153,10 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
             }
             int32_t rows[K7_KEYS / 16];
 #pragma unroll
-            for (int h = 0; h < K7_KEYS / 16; ++h) rows[h] = __shfl_sync(0xffffffffu, row, h);
+            for (int h = 0; h < K7_KEYS / 16; ++h) rows[h] = __shfl_sync(0xffffffffu, row, in_batch + h);
             if (lane == 0) {
               mbar_expect_tx(full + stage * 8, S::KV_BYTES);
+              mbar_arrive_many(full + stage * 8, 32);
 #pragma unroll
               for (int h = 0; h < K7_KEYS / 16; ++h) {
                 if (h & (p.big_box - 1)) continue;
@@ -1162,11 +1178,12 @@ __global__ void __launch_bounds__(K7_THREADS, 1) k7_attention_kernel(
                           pool + static_cast<int64_t>(max(from, 0)) * D, from >= 0);
               }
             }
+            k7_copies_arrive(full + stage * 8);
           }
-          k7_copies_arrive(full + stage * 8);
         }
         x = next;
         pages = next_pages;
+        ahead = next_ahead;
         there = next_there;
         ++piece;
       }
