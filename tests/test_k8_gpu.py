@@ -240,3 +240,35 @@ def test_many_sequences(cuda_device, n):
     starts = torch.randint(0, 4, (n,), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
     _run(c, cuda_device, starts)
     _run(c, cuda_device, None, reduction="sequence", return_grad=False)
+
+
+@pytest.mark.parametrize("seed", range(4))
+def test_ratio_keeps_its_bits(cuda_device, seed):
+    """fp32 gradients of rows with two large logits; the others' exponentials (below e^-1000) add nothing,
+    exactly.  So the sum s is off by an ex2 (2^-22) and three roundings, which reach the gradient twice,
+    by log s in the ratio and by the division; log s itself by half a step of a number below 1 (2^-25);
+    expf and the second ex2 by 2^-22 each; the exponent's one rounding, slope, weight and products by nine
+    roundings: 2 (2^-22 + 3 2^-24) + 2^-25 + 2 2^-22 + 9 2^-24 < 2^-19, relative to slope times p (or
+    times 1 at the target, where 1 - p may cancel).  (Roundings at the size of the logits, 2000 after
+    the division, would be 2^-14 each.)"""
+    import tome_b200
+    n, length, vocab, T = 2, 8, 5000, 0.5
+    g = torch.Generator().manual_seed(seed)
+    x = 2 * torch.randn((n, length, vocab), generator=g)
+    ids = torch.randint(0, vocab, (n, length), generator=g, dtype=torch.int32)
+    ids.clamp_(min=1)
+    x.scatter_(-1, ids.long()[..., None], 1000.0)                    # the target stands out, far from 0
+    x[..., 0] = 1000.25
+    lp = torch.log_softmax(x.double() / T, -1).gather(-1, ids.long()[..., None])[..., 0]
+    old = (lp - 0.05 * torch.randn((n, length), generator=g).double()).float()
+    adv, lengths = torch.tensor([1.0, -1.0]), torch.full((n,), length, dtype=torch.int32)
+    _, _, grad = tome_b200.grpo_policy_loss(*(t.to(cuda_device) for t in (x, ids, old, adv, lengths)), T, check=True)
+    want = step.policy_loss(x, ids, old, adv, lengths, T)[2]
+    slope = want.gather(-1, ids.long()[..., None]).abs() / (1 - lp.exp())[..., None]
+    one = torch.zeros_like(want).scatter_(-1, ids.long()[..., None], 1.0)
+    p = torch.softmax(x.double() / T, -1)
+    rel = 2.0 ** -19
+    away = (x.double().amax(-1, keepdim=True) - x.double()) / T      # the exponent's size, rounded twice
+    tol = slope * (p + one) * (rel + 2.0 ** -22 * away) + 2.0 ** -126
+    off = (grad.cpu().double() - want).abs()
+    assert bool((off <= tol).all()), float((off / tol).max())
