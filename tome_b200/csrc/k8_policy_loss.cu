@@ -15,6 +15,12 @@
 // of bulk copies; pass 2 fetches the part again while it is still in L2, so that HBM sees the
 // logits once and the gradient once.  Rows outside the windows are not read; their gradient is
 // written as zeros by the same CTAs.
+//
+// Measured (CUDA-graph replay, vocabulary 151936, windows of random length): 32 x 256 bf16 rows 680 to
+// 720 us (box to box), 5.2 to 5.5 TB/s (0.79 to 0.83 of a copy); 24 fp32 rows 12.4 to 13.2 us.  1080
+// bf16 rows of 50257 50 us, 3.3 TB/s: few rows per cluster, which do not
+// come out even.  Dealing the rows of the windows evenly among the clusters by a search in the prefix
+// sums of their lengths took 46 to 48 us there, but 3.5 % more with many rows and 5 % with few.
 #include "k1_common.cuh"
 #include "row_geom.cuh"
 
