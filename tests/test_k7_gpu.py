@@ -304,3 +304,51 @@ def test_more_random_batches(cuda_device, seed):
     kv = pick(1, 2, 5)
     _run(_case(seed, groups, lengths, prefix, pick(8, 13, 16, 32), kv * pick(1, 2, 4, 7, 8), kv, pick(64, 128),
                pick(torch.bfloat16, torch.float16)), cuda_device)
+
+
+@pytest.mark.parametrize("block", [16, 32, 48, 64, 80, 128, 192])
+@pytest.mark.parametrize("heads,kv", [(8, 2), (32, 1)])
+def test_big_tiles_with_missing_and_repeated_pages(cuda_device, block, heads, kv):
+    """More than sixteen rows a KV head and many tiles: pages that do not exist (their tile is copied row by
+    row, between tiles of tensor copies), pages named twice, an end inside a page."""
+    import tome_b200
+    c = _case(block, [8], [33, 0, 200, 64, 1, 90, 5, 130], [3001], block, heads, kv, 128, torch.bfloat16)
+    table = c["prefix_tables"]
+    used = (3001 + block - 1) // block
+    for i in {1, used // 3, used // 2, used - 1}:
+        table[0, i] = -1 if i % 2 else c["k_pool"].shape[0]
+    table[0, used // 4] = table[0, 0]
+    c["tables"][2, 0] = table[0, 0]
+    out, lse = tome_b200.shared_prefix_attention(*_dev(c, cuda_device), return_lse=True)
+    with pytest.raises(tome_b200.TomeRuntimeError, match="block-table"):
+        tome_b200.check_device_status(cuda_device)
+    _compare(c, out, lse)
+
+
+@pytest.mark.parametrize("block", [32, 64])
+def test_what_lies_behind_a_big_prefix_is_not_read(cuda_device, block):
+    c = _case(block, [12], [7] * 12, [block * 9 + 5], block, 8, 2, 64, torch.float16)
+    want, want_lse = _run(c, cuda_device)
+    last = int(c["prefix_tables"][0, 9])
+    for pool in (c["k_pool"], c["v_pool"]):
+        pool[last, :, 5:] = float("nan")
+        named = torch.cat([c["prefix_tables"].reshape(-1), c["tables"].reshape(-1)]).long()
+        rest = torch.ones(pool.shape[0], dtype=torch.bool)
+        rest[named] = False
+        pool[rest] = float("inf")
+    import tome_b200
+    got, got_lse = tome_b200.shared_prefix_attention(*_dev(c, cuda_device), return_lse=True, check=True)
+    assert torch.equal(got, want) and torch.equal(got_lse, want_lse)
+
+
+def test_as_many_sequences_and_groups_as_a_call_takes(cuda_device):
+    import tome_b200
+    g = torch.Generator().manual_seed(3)
+    lens = torch.randint(0, 20, (2048,), generator=g).tolist()
+    prefix = torch.randint(0, 70, (512,), generator=g).tolist()
+    c = _case(31, [4] * 512, lens, prefix, 16, 8, 1, 64, torch.bfloat16)  # 32 rows a group: all prefixes big
+    _run(c, cuda_device)
+    more = dict(c, q=torch.cat([c["q"], c["q"][:1]]), tables=torch.cat([c["tables"], c["tables"][:1]]),
+                lengths=torch.cat([c["lengths"], c["lengths"][:1]]))
+    with pytest.raises(ValueError):
+        tome_b200.shared_prefix_attention(*_dev(more, cuda_device))
